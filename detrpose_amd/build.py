@@ -36,6 +36,8 @@ def _hipcc() -> str:
 def _flags() -> list[str]:
     extra = os.environ.get("DETRPOSE_EXTRA_FLAGS", "").split()
     return ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
+            # no packed f32 instructions: some forms of v_pk_add / mul / fma_f32 have given wrong results on MI355X
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
             "-I", os.path.join(REPO, "include")] + extra
 
 
@@ -116,6 +118,10 @@ def build(force: bool = False, verbose: bool = False, variant: str = "") -> str:
     hipcc = _hipcc()
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
     deps = glob.glob(os.path.join(CSRC, "*.h")) + [os.path.join(REPO, "include", "detrpose_hip.h")]
+    # objects compiled with other flags are stale whatever their age
+    stamp, flags = os.path.join(BUILD, "flags.txt"), " ".join(_flags())
+    if not os.path.exists(stamp) or open(stamp).read() != flags:
+        force = True
     jobs = []
     objs = []
     for s in srcs:
@@ -131,6 +137,8 @@ def build(force: bool = False, verbose: bool = False, variant: str = "") -> str:
                     sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
                 if r.returncode:
                     raise RuntimeError(f"hipcc failed on {cmd[-3]}")
+    with open(stamp, "w") as f:
+        f.write(flags)
     hobj, hnew = _hash_object(BUILD)
     objs.append(hobj)
     if jobs or hnew or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
