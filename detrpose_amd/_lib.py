@@ -193,6 +193,13 @@ _SIGS = {
     "dp_upsample2x": (i32, [vp, i64, i32, i32, i32, i32, i32, vp, i64, i32, i32, i32, vp]),
     "dp_axpby_rows": (i32, [vp, i64, vp, i64, f32, vp, i64, f32, i32, i32, i32, i32, vp]),
     "dp_act_bwd": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp]),
+    # token sequences (csrc/rms_norm.hip), gradients of separate tensors (grad_clip.hip)
+    "dp_rms_norm": (i32, [vp, vp, vp, vp, i64, vp, i64, vp, i32, f32, i32, i32, i32, vp]),
+    "dp_rms_norm_e4m3": (i32, [vp, vp, vp, vp, i64, vp, i64, vp, i32, f32, i32, i32, i32, vp]),
+    "dp_rms_norm_bwd_ws_floats": (i64, [i32, i32, i32]),
+    "dp_rms_norm_bwd": (i32, [vp, vp, vp, i64, vp, vp, i64, vp, i64, vp, i32, vp, i64, i32, i32, i32, vp]),
+    "dp_grad_clip_ws_bytes": (i64, [i32]),
+    "dp_grad_clip": (i32, [vp, vp, vp, i32, f32, vp, vp, i64, i32, vp, i64, vp]),
 }
 
 EXPORTED = tuple(k for k in _SIGS)

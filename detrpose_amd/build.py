@@ -41,10 +41,12 @@ def _flags() -> list[str]:
             "-I", os.path.join(REPO, "include")] + extra
 
 
-# translation units no inference plan launches from (the training step's kernels): left out of
-# source_hash, so a training-only change keeps the inference line's committed PMC profile valid
+# translation units no inference plan launches from (the training step's kernels, the token-sequence
+# operators): left out of source_hash, so a training-only change keeps the inference line's
+# committed PMC profile valid
 TRAINING_ONLY = {"backbone_train.hip", "criterion.hip", "encoder_train.hip", "gemm.hip", "msda_train.hip",
-                 "train.hip", "train_attn.hip", "preprocess.hip"}
+                 "train.hip", "train_attn.hip", "preprocess.hip", "rms_norm.hip", "grad_clip.hip", "packed_attn_fwd.hip",
+                 "packed_attn_bwd.hip", "packed_attn.h"}
 
 
 def source_hash() -> str:

@@ -734,6 +734,36 @@ int dp_maxpool2x2_pad_rb_bwd(const void* x, int64_t x_bstride, int32_t x_pstride
                              int64_t dout_bstride, int32_t dout_pstride, int32_t batch, int32_t h, int32_t w, int32_t c,
                              void* dx, int64_t dx_bstride, int32_t dx_pstride, int32_t dtype, void* stream);
 
+/* ---- Token sequences and gradients of separate tensors. Callers: detrpose_amd/{attention,norm,
+ * gradients}.py. */
+
+/* Root-mean-square norm over rows of c elements: r = x (+ res, rounded to dtype and written when r is
+ * not NULL), rstd = 1 / sqrt(mean r^2 + eps) (f32 [rows], written when not NULL), y = r rstd weight.
+ * x / res rows ld_x / ld_res apart, y / r contiguous; weight [c] f32 or dtype. c up to 8192 (f32),
+ * 16384 (bf16); rows need only their element's alignment. */
+int dp_rms_norm(void* y, void* r, float* rstd, const void* x, int64_t ld_x, const void* res, int64_t ld_res,
+                const void* weight, int32_t w_dtype, float eps, int32_t rows, int32_t c, int32_t dtype, void* stream);
+/* The same with an 8-bit output: y e4m3 [rows][c] = norm / scale, scale f32 [rows] = max |norm| / 448. */
+int dp_rms_norm_e4m3(void* y, float* scale, void* r, const void* x, int64_t ld_x, const void* res, int64_t ld_res,
+                     const void* weight, int32_t w_dtype, float eps, int32_t rows, int32_t c, int32_t dtype,
+                     void* stream);
+/* Backward of dp_rms_norm from r (its x without a residual) and rstd: dx (the gradient of x and of res)
+ * = the norm's (+ dres, the gradient that reached r, NULL = none); dweight [c] of w_dtype, summed in a
+ * fixed order through ws (dp_rms_norm_bwd_ws_floats floats). */
+int64_t dp_rms_norm_bwd_ws_floats(int32_t rows, int32_t c, int32_t dtype);
+int dp_rms_norm_bwd(void* dx, void* dweight, const void* r, int64_t ld_r, const float* rstd, const void* dy,
+                    int64_t ld_dy, const void* dres, int64_t ld_dres, const void* weight, int32_t w_dtype, float* ws,
+                    int64_t ws_floats, int32_t rows, int32_t c, int32_t dtype, void* stream);
+
+/* clip_grad_norm_ over many tensors (src/solver/engine.py:78-89): ptr / n / dtype are host arrays of
+ * count device pointers, element counts and types (read before the call returns); *norm (device f32) =
+ * sqrt(sum of all squares), and every element is multiplied by min(1, max_norm / (norm + 1e-6)), in
+ * place, or, when out is not NULL, into out (out_n = all elements, one tensor behind the other). No
+ * two tensors share memory (checked). Deterministic. ws: dp_grad_clip_ws_bytes(count) bytes. */
+int64_t dp_grad_clip_ws_bytes(int32_t count);
+int dp_grad_clip(void* const* ptr, const int64_t* n, const int32_t* dtype, int32_t count, float max_norm, float* norm,
+                 void* out, int64_t out_n, int32_t out_dtype, void* ws, int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
