@@ -81,6 +81,18 @@ class RowCopyDesc(C.Structure):
                 ("rows", i32), ("n", i32)]
 
 
+class PackedAttn(C.Structure):
+    """Mirror of dp_packed_attn."""
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("out", vp), ("lse", vp),
+                ("q_row", i64), ("q_head", i64), ("k_row", i64), ("k_head", i64), ("v_row", i64), ("v_head", i64),
+                ("o_row", i64), ("o_head", i64), ("cu_q", vp), ("cu_k", vp),
+                ("nseq", i32), ("tq", i32), ("tk", i32), ("heads", i32), ("kv_heads", i32), ("dim", i32),
+                ("causal", i32), ("fill_tail", i32), ("scale", f32), ("dtype", i32),
+                ("bias", vp), ("bias_dtype", i32), ("buckets", i32), ("both", i32), ("edge", i32 * 64),
+                ("ws", vp), ("ws_bytes", i64),
+                ("dout", vp), ("g_row", i64), ("g_head", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dbias", vp)]
+
+
 def rowmap(base=0, group=1, stride_g=0, stride_r=0) -> RowMap:
     return RowMap(int(base), int(group), int(stride_g), int(stride_r))
 
@@ -193,7 +205,10 @@ _SIGS = {
     "dp_upsample2x": (i32, [vp, i64, i32, i32, i32, i32, i32, vp, i64, i32, i32, i32, vp]),
     "dp_axpby_rows": (i32, [vp, i64, vp, i64, f32, vp, i64, f32, i32, i32, i32, i32, vp]),
     "dp_act_bwd": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp]),
-    # token sequences (csrc/rms_norm.hip), gradients of separate tensors (grad_clip.hip)
+    # token sequences (csrc/packed_attn_*.hip, rms_norm.hip), gradients of separate tensors (grad_clip.hip)
+    "dp_packed_attn_ws_bytes": (i64, [C.POINTER(PackedAttn), i32]),
+    "dp_packed_attn_fwd": (i32, [C.POINTER(PackedAttn), vp]),
+    "dp_packed_attn_bwd": (i32, [C.POINTER(PackedAttn), vp]),
     "dp_rms_norm": (i32, [vp, vp, vp, vp, i64, vp, i64, vp, i32, f32, i32, i32, i32, vp]),
     "dp_rms_norm_e4m3": (i32, [vp, vp, vp, vp, i64, vp, i64, vp, i32, f32, i32, i32, i32, vp]),
     "dp_rms_norm_bwd_ws_floats": (i64, [i32, i32, i32]),

@@ -1,0 +1,295 @@
+// Shared pieces of attention over packed sequences (packed_attn_fwd.hip, packed_attn_bwd.hip).
+//
+// Rows. The query heads that share a key head are folded into the rows: row r of a (sequence, key
+// head) is query r / G, head r % G of the group (G = heads / kv_heads), so one tile of rows reads a key
+// tile once for all of them, and the sums over a group's heads in dk / dv are plain row sums.
+//
+// Matrix layouts (v_mfma_f32_32x32x16_bf16, v_mfma_f32_32x32x2_f32; lane l, h = l >> 5): the A
+// operand's row and the B operand's column are l & 31, the accumulator's column is l & 31 and its
+// register i holds row 8 (i / 4) + 4 h + i % 4. Every product is arranged so that an accumulator is
+// the next product's B operand as it stands: S^T = K Q^T has queries in columns, and the contraction
+// of O^T = V^T P^T runs over the accumulator's rows, the slot (h, j) of a 16-row step standing for
+// row 16 m + 8 (j / 4) + 4 h + j % 4 on both sides. In bf16 the other side, V^T, is read from the
+// row-major tile with the transposing LDS read (4 rows x 16 columns per 16 lanes), in f32 with one
+// 4-byte read per step.
+//
+// Tiles. Rows of DP elements (dim padded to 32, 64 or 128; the padding reads as zero), filled by
+// direct HBM -> LDS loads whose buffer descriptor returns zero for rows outside the sequence: what
+// lies there (another sequence, an unwritten cache row) never enters a product. A row's 16-byte chunks
+// are permuted by its number (swz) so that both read patterns spread over all banks; the permutation
+// is applied to the global address, because the LDS side of such a load is contiguous per wave.
+#pragma once
+#include "common.h"
+#include "conv_lds.h"
+
+namespace dppa {
+
+using dpconv::dma16;
+using dpconv::i32x4;
+using dpconv::make_rsrc;
+using dpconv::OOB;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int NT = 256;     // threads of a block: 4 waves, 32 rows (or keys) each
+constexpr int BM = 128;     // rows (keys, in the dk / dv kernel) of a block
+
+// what a kernel needs to know; strides in elements
+struct Args {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+  const int32_t *cu_q, *cu_k;
+  int nseq, tq, tk, hkv, group, dim, causal, tiles;
+  float scale;
+  // bias
+  const void* bias;
+  int bias_f32, buckets, both, nedge;
+  int32_t edge[64];
+  // backward
+  const void* dout;
+  int64_t g_row, g_head;
+  void *dq, *dk, *dv;
+  float* dsum;
+  float* dbias_part;
+};
+
+template <typename T> struct Tr;
+template <> struct Tr<bf16_t> { static constexpr int VN = 8; };
+template <> struct Tr<float> { static constexpr int VN = 4; };
+
+template <typename T, int DP>
+struct Tile {
+  static constexpr int VN = Tr<T>::VN;          // elements of a 16-byte chunk
+  static constexpr int CPR = DP / VN;           // chunks of a row
+  static constexpr int RB = DP * (int)sizeof(T);
+  static constexpr int KS = CPR / 2;            // chunk pairs: the steps of a product over dim
+  static constexpr int ND = DP / 32;            // 32-wide column tiles
+  // the chunk permutation of a row: consecutive rows' equal chunks, and the chunk pairs of 4
+  // consecutive rows, land on different 16-byte slots of the 128-byte bank line
+  __device__ static __forceinline__ int swz(int row) {
+    return CPR >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : (((row & 2)) | ((row >> 2) & 1));
+  }
+};
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// one chunk-pair step of a product over dim: 16 elements in bf16, 8 in f32
+template <typename T>
+__device__ __forceinline__ f32x16 mma_step(const u32x4& a, const u32x4& b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  } else {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// tile rows (32 sub + l & 31) x the lane's column fragments
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 rows_mma(const char* tile, int sub, int lane, const u32x4 (&b)[Tile<T, DP>::KS]) {
+  using TL = Tile<T, DP>;
+  const int row = lane & 31, h = lane >> 5;
+  const char* base = tile + (32 * sub + row) * TL::RB;
+  const int f = TL::swz(row);
+  f32x16 c = zero16();
+#pragma unroll
+  for (int s = 0; s < TL::KS; ++s) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(base + (((2 * s + h) ^ f) << 4));
+    c = mma_step<T>(a, b[s], c);
+  }
+  return c;
+}
+
+// acc[t] += tile^T (columns 32 t ...) x p, contracted over the tile's rows 32 sub .. 32 sub + 31
+template <typename T, int DP>
+__device__ __forceinline__ void cols_mma(const char* tile, int sub, int lane, const f32x16& p,
+                                         f32x16 (&acc)[Tile<T, DP>::ND]) {
+  using TL = Tile<T, DP>;
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    const int q4 = (lane & 15) >> 2, p4 = lane & 3, dg = (lane >> 4) & 1;
+    const int r = 4 * h + q4;   // row & 7 of every row this lane addresses
+    const int f = TL::swz(r);
+    const char* base = tile + (32 * sub + r) * TL::RB + (p4 & 1) * 8;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      bf16x8 b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[j] = (bf16_t)p[8 * m + j];
+#pragma unroll
+      for (int t = 0; t < TL::ND; ++t) {
+        const char* at = base + 16 * m * TL::RB + (((4 * t + 2 * dg + (p4 >> 1)) ^ f) << 4);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
+        const s16x4 hi =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * TL::RB));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        const s16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[t], 0, 0, 0);
+      }
+    }
+  } else {
+    const int c = (lane & 31) >> 2, w = (lane & 3) * 4;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = 8 * (i / 4) + 4 * h + (i & 3);
+      const char* base = tile + (32 * sub + row) * TL::RB + w;
+      const int f = TL::swz(row);
+#pragma unroll
+      for (int t = 0; t < TL::ND; ++t) {
+        const float a = *reinterpret_cast<const float*>(base + (((8 * t + c) ^ f) << 4));
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[t], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// ROWS rows into a tile: row r from rsrc + off(r) bytes, zero where off is negative or past dim
+template <typename T, int DP, int ROWS, typename OFF>
+__device__ __forceinline__ void stage(const i32x4& rsrc, char* tile, int dim, OFF off) {
+  using TL = Tile<T, DP>;
+  static_assert(ROWS * TL::CPR % NT == 0, "whole passes");
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int it = 0; it < ROWS * TL::CPR / NT; ++it) {
+    const int slot = it * NT + threadIdx.x;
+    const int row = slot / TL::CPR, c = (slot % TL::CPR) ^ TL::swz(row);
+    const int o = off(row);
+    dma16(rsrc, tile + (it * NT + wave * 64) * 16, o >= 0 && c * TL::VN < dim ? o + c * 16 : OOB);
+  }
+}
+
+// the lane's fragments of one global row as a B operand (zero when !ok and past dim)
+template <typename T, int DP>
+__device__ __forceinline__ void load_frags(const T* row, bool ok, int dim, int h, u32x4 (&f)[Tile<T, DP>::KS]) {
+#pragma unroll
+  for (int s = 0; s < Tile<T, DP>::KS; ++s) {
+    const int e = (2 * s + h) * Tr<T>::VN;
+    f[s] = ok && e < dim ? *reinterpret_cast<const u32x4*>(row + e) : u32x4{0, 0, 0, 0};
+  }
+}
+
+// both halves of the wave get a (op) b of lanes l and l ^ 32
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// everything issued to LDS so far has landed, for every wave of the block
+__device__ __forceinline__ void tile_barrier() {
+  dpconv::wait_vmcnt<0>();
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------- which sequence a block works on
+// The lengths are on the device only: a launch has as many blocks as the packed total allows at
+// most, and every wave finds its block's (sequence, tile) by a scan over the sequences, 64 at a time.
+// nseq counts one more when the rows behind the last sequence are an item of their own (tail).
+struct Item { int b, tile, start, len; };
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// rows_of(len) rows of `per` a tile
+__device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total, int mult, int per, bool tail, int idx,
+                                          Item& it) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  const int n = nseq + (tail ? 1 : 0);
+  for (int base = 0; base < n; base += 64) {
+    const int b = base + lane;
+    int start = 0, len = 0;
+    if (b < n) {
+      start = b ? clampi(cu[b], 0, total) : 0;
+      len = max(0, (b < nseq ? clampi(cu[b + 1], 0, total) : total) - start);
+    }
+    const int cnt = (len * mult + per - 1) / per;
+    int inc = cnt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(inc, o, 64);
+      if (lane >= o) inc += u;
+    }
+    const int all = __shfl(inc, 63, 64);
+    if (idx < before + all) {
+      const unsigned long long m = __ballot(idx < before + inc);
+      const int l = __ffsll((long long)m) - 1;
+      it.b = __builtin_amdgcn_readfirstlane(base + l);
+      it.tile = __builtin_amdgcn_readfirstlane(idx - before - __shfl(inc - cnt, l, 64));
+      it.start = __builtin_amdgcn_readfirstlane(__shfl(start, l, 64));
+      it.len = __builtin_amdgcn_readfirstlane(__shfl(len, l, 64));
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+// start and length of sequence b (nothing for the tail)
+__device__ __forceinline__ void seq_of(const int32_t* cu, int nseq, int total, int b, int& start, int& len) {
+  start = b && b < nseq ? clampi(cu[b], 0, total) : 0;
+  len = b < nseq ? max(0, clampi(cu[b + 1], 0, total) - start) : 0;
+  start = __builtin_amdgcn_readfirstlane(start);
+  len = __builtin_amdgcn_readfirstlane(len);
+}
+
+// ---------------------------------------------------------------- relative position bias
+// LDS: tab[g][bucket] f32 of the group's heads, then lut[n] = bucket of distance n, n <= last (the
+// distance from which on every one is in the last bucket).
+struct Bias {
+  const float* tab;
+  const uint8_t* lut;
+  int nb, last, half, both;
+  __device__ __forceinline__ int bucket(int rel) const {
+    const int n = min(both ? abs(rel) : max(-rel, 0), last);
+    return lut[n] + (rel > 0 ? half : 0);
+  }
+  // the bucket that every distance in [lo, hi] falls into, or -1 (there may be several)
+  __device__ __forceinline__ int one_bucket(int lo, int hi) const {
+    if (hi <= -last) return lut[last];
+    if (both ? lo >= last : lo >= 0) return both ? lut[last] + half : 0;
+    return -1;
+  }
+};
+
+static inline int bias_lds(const Args& a) {
+  return a.bias ? a.group * a.buckets * 4 + ((a.nedge ? a.edge[a.nedge - 1] : 0) + 1 + 15) / 16 * 16 : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ Bias bias_setup(const Args& a, char* lds, int kvh) {
+  float* tab = reinterpret_cast<float*>(lds);
+  uint8_t* lut = reinterpret_cast<uint8_t*>(tab + a.group * a.buckets);
+  const int heads = a.hkv * a.group;
+  for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) {
+    const int g = i / a.buckets, b = i - g * a.buckets;
+    const int64_t at = (int64_t)b * heads + kvh * a.group + g;
+    tab[i] = a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[at] : to_f32(reinterpret_cast<const T*>(a.bias)[at]);
+  }
+  const int last = a.nedge ? a.edge[a.nedge - 1] : 0;
+  for (int n = threadIdx.x; n <= last; n += NT) {
+    int b = 0;
+    for (int e = 0; e < a.nedge; ++e) b += a.edge[e] <= n;
+    lut[n] = (uint8_t)b;
+  }
+  __syncthreads();
+  return Bias{tab, lut, a.buckets, last, a.both ? a.buckets / 2 : 0, a.both};
+}
+
+}  // namespace dppa

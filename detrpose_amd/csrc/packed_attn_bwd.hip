@@ -1,0 +1,415 @@
+// Attention over packed sequences, backward (packed_attn.h has the layouts).
+//
+//   p = exp(s - lse), dp = dO V^T, D = sum_d dO O, ds = p (dp - D)
+//   dQ = scale ds K, dK = scale ds^T Q, dV = p^T dO, dbias[bucket][head] = sum of ds in the bucket
+//
+// Two kernels, each owner of what it writes, so nothing is added atomically and equal inputs give
+// equal bits: packed_bwd_q_kernel walks the keys of a tile of 128 rows (S^T, dP^T, dQ^T: three products)
+// and stores D; packed_bwd_kv_kernel walks the rows (all heads of the group, so grouped heads are summed
+// in the accumulators) of a tile of 128 keys (S, dP, dV^T, dK^T: four products). Two of the seven products
+// are done twice in exchange. p and ds are rounded to bf16 for their products, as p in the forward.
+//
+// The table's gradient comes from the first kernel: each lane owns one row (one head), so it adds its
+// ds into its own LDS bins [bucket][thread] (a 4-byte add with no other lane at that address; one add
+// per tile where the whole tile lies in one bucket); the block then adds the bins of a head's rows and
+// writes one part per block, and packed_dbias_kernel adds the parts, all in fixed orders.
+#include "packed_attn.h"
+
+int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what, bool backward);
+
+namespace {
+using namespace dppa;
+
+template <typename T, int DP, int BN, bool BIAS>
+__global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int TB = BN * TL::RB, NS = BN / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int kvh = blockIdx.x % a.hkv, tile = a.tiles - 1 - blockIdx.x / a.hkv;
+  const int heads = a.hkv * a.group;
+  float* part = BIAS ? a.dbias_part + ((int64_t)tile * a.hkv + kvh) * a.group * a.buckets : nullptr;
+  Item it;
+  if (!find_item(a.cu_q, a.nseq, a.tq, a.group, BM, true, tile, it)) {
+    if constexpr (BIAS)
+      for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) part[i] = 0.f;
+    return;
+  }
+  const int q0 = it.start, lq = it.len;
+  int k0, lk;
+  seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
+  const int off = lk - lq, rows = lq * a.group, row0 = it.tile * BM;
+  const int first = row0 + 32 * wave, r = first + (lane & 31);
+  const bool ok = r < rows;
+  const int rc = min(r, rows - 1), pos = rc / a.group, g = rc - pos * a.group, head = kvh * a.group + g;
+  auto limit = [&](int row) {
+    return a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
+  };
+  const int lim = limit(r), wmin = limit(first), wmax = first < rows ? limit(first + 31) : 0;
+  const int nt = (limit(row0 + BM - 1) + BN - 1) / BN;
+  Bias bias{};
+  float* bins = nullptr;
+  if constexpr (BIAS) {
+    bins = reinterpret_cast<float*>(smem + 4 * TB);
+    for (int b = 0; b < a.buckets; ++b) bins[b * NT + threadIdx.x] = 0.f;   // the thread's own
+    bias = bias_setup<T>(a, smem + 4 * TB + a.buckets * NT * 4, kvh);
+    bins += threadIdx.x;
+  }
+
+  const int64_t at = (int64_t)(q0 + pos) * heads + head;
+  u32x4 qf[TL::KS], gf[TL::KS];
+  load_frags<T, DP>((const T*)a.q + (int64_t)(q0 + pos) * a.q_row + head * a.q_head, ok, a.dim, h, qf);
+  load_frags<T, DP>((const T*)a.dout + (int64_t)(q0 + pos) * a.g_row + head * a.g_head, ok, a.dim, h, gf);
+  float D = 0.f;
+  {
+    u32x4 of[TL::KS];
+    load_frags<T, DP>((const T*)a.out + (int64_t)(q0 + pos) * a.o_row + head * a.o_head, ok, a.dim, h, of);
+#pragma unroll
+    for (int s = 0; s < TL::KS; ++s) {
+      const T* x = reinterpret_cast<const T*>(&of[s]);
+      const T* y = reinterpret_cast<const T*>(&gf[s]);
+#pragma unroll
+      for (int e = 0; e < TL::VN; ++e) D = fmaf(to_f32(x[e]), to_f32(y[e]), D);
+    }
+    D = half_sum(D);
+  }
+  if (ok && h == 0) a.dsum[at] = D;
+  const float lse = ok ? a.lse[at] : INFINITY;
+
+  auto fetch = [&](int j) {
+    char* buf = smem + (j & 1) * 2 * TB;
+    const int key0 = j * BN, left = lk - key0;
+    const i32x4 rk = make_rsrc((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head);
+    const i32x4 rv = make_rsrc((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head);
+    const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
+    stage<T, DP, BN>(rk, buf, a.dim, [&](int row) { return row < left ? row * ks : -1; });
+    stage<T, DP, BN>(rv, buf + TB, a.dim, [&](int row) { return row < left ? row * vs : -1; });
+  };
+
+  const float c = a.scale * LOG2E;
+  f32x16 dq[TL::ND];
+#pragma unroll
+  for (int t = 0; t < TL::ND; ++t) dq[t] = zero16();
+
+  dpconv::wait_vmcnt<0>();   // the row loads above, so that the loop's waits count tiles only
+  if (nt > 0) fetch(0);
+  for (int j = 0; j < nt; ++j) {
+    tile_barrier();
+    if (j + 1 < nt) fetch(j + 1);
+    const char* buf = smem + (j & 1) * 2 * TB;
+    const int key0 = j * BN;
+    if (key0 >= wmax) continue;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      const int k32 = key0 + 32 * u;
+      if (k32 >= wmax) break;
+      f32x16 s = rows_mma<T, DP>(buf, u, lane, qf);
+      const f32x16 dp = rows_mma<T, DP>(buf + TB, u, lane, gf);
+      int one = -1;
+      if constexpr (BIAS) {
+        const int pl = min(first + 31, rows - 1) / a.group + off, pf = first / a.group + off;
+        one = bias.one_bucket(k32 - pl, k32 + 31 - pf);
+        const float* tab = bias.tab + g * bias.nb;
+        if (one >= 0) {
+          const float b = tab[one];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], a.scale, b);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[i] = fmaf(s[i], a.scale, tab[bias.bucket(k32 + 8 * (i / 4) + 4 * h + (i & 3) - pos - off)]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(BIAS ? (s[i] - lse) * LOG2E : fmaf(s[i], c, -lse));
+        s[i] = p * (dp[i] - D);
+      }
+      if (k32 + 32 > wmin) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (k32 + 8 * (i / 4) + 4 * h + (i & 3) >= lim) s[i] = 0.f;
+      }
+      if constexpr (BIAS) {
+        if (one >= 0) {
+          float t = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) t += s[i];
+          bins[one * NT] += t;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            __hip_atomic_fetch_add(bins + bias.bucket(k32 + 8 * (i / 4) + 4 * h + (i & 3) - pos - off) * NT, s[i],
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
+      cols_mma<T, DP>(buf, u, lane, s, dq);
+    }
+  }
+
+  if (ok) {
+    T* op = (T*)a.dq + at * a.dim;
+#pragma unroll
+    for (int t = 0; t < TL::ND; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 32 * t + 8 * e + 4 * h;
+        if (d < a.dim) {
+          typedef T T4 __attribute__((ext_vector_type(4)));
+          T4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(dq[t][4 * e + i] * a.scale);
+          *reinterpret_cast<T4*>(op + d) = w;
+        }
+      }
+  }
+  if constexpr (BIAS) {
+    __syncthreads();
+    const float* all = reinterpret_cast<const float*>(smem + 4 * TB);
+    for (int p = threadIdx.x; p < a.group * a.buckets; p += NT) {
+      const int pg = p / a.buckets, b = p - pg * a.buckets;
+      int rr = (pg - row0 % a.group + a.group) % a.group;   // the block's first row of this head
+      float t = 0.f;
+      for (; rr < min(BM, rows - row0); rr += a.group) {
+        const float* x = all + b * NT + (rr >> 5) * 64 + (rr & 31);
+        t += x[0] + x[32];
+      }
+      part[p] = t;
+    }
+  }
+}
+
+// dbias[bucket][head] = sum over tiles of the parts, in order: one block per head
+template <typename TB>
+__global__ __launch_bounds__(NT) void packed_dbias_kernel(TB* __restrict__ out, const float* __restrict__ part,
+                                                          int tiles, int hkv, int group, int buckets) {
+  __shared__ float sm[NT];
+  const int head = blockIdx.x, kvh = head / group, g = head - kvh * group;
+  const int b = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  float s = 0.f;
+  if (b < buckets)
+    for (int t = slice; t < tiles; t += NT / 64)
+      s += part[(((int64_t)t * hkv + kvh) * group + g) * buckets + b];
+  sm[threadIdx.x] = s;
+  __syncthreads();
+  if (slice == 0 && b < buckets)
+    out[(int64_t)b * hkv * group + head] = from_f32<TB>((sm[b] + sm[64 + b]) + (sm[128 + b] + sm[192 + b]));
+}
+
+template <typename T, int DP, int BR, bool BIAS>
+__global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kernel(const Args a) {
+  using TL = Tile<T, DP>;
+  constexpr int TB = BR * TL::RB, NS = BR / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  // per row of a tile: lse, D, and (for the bias) its position and head; two buffers, written a tile ahead
+  float* lse_s = reinterpret_cast<float*>(smem + 4 * TB);
+  float* dsum_s = lse_s + 2 * BR;
+  int* pos_s = reinterpret_cast<int*>(dsum_s + 2 * BR);
+  int* head_s = pos_s + 2 * BR;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int kvh = blockIdx.x % a.hkv;
+  const int heads = a.hkv * a.group;
+  Item it;
+  if (!find_item(a.cu_k, a.nseq, a.tk, 1, BM, true, blockIdx.x / a.hkv, it)) return;
+  const int k0 = it.start, lk = it.len;
+  int q0, lq;
+  seq_of(a.cu_q, a.nseq, a.tq, it.b, q0, lq);
+  const int off = lk - lq, rows = lq * a.group;
+  const int first = it.tile * BM + 32 * wave, key = first + (lane & 31);
+  const bool ok = key < lk;
+  // the first row that sees a key
+  auto sees = [&](int kk) { return a.causal ? max(0, kk - off) * a.group : 0; };
+  const int mine = sees(key), wfirst = sees(first), wlast = sees(min(first + 31, lk - 1));
+  Bias bias{};
+  if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB + 16 * BR * 2, kvh);
+
+  u32x4 kf[TL::KS], vf[TL::KS];
+  load_frags<T, DP>((const T*)a.k + (int64_t)(k0 + min(key, lk - 1)) * a.k_row + kvh * a.k_head, ok, a.dim, h, kf);
+  load_frags<T, DP>((const T*)a.v + (int64_t)(k0 + min(key, lk - 1)) * a.v_row + kvh * a.v_head, ok, a.dim, h, vf);
+
+  const int start = sees(it.tile * BM) / 32 * 32;
+  const int nt = rows > start ? (rows - start + BR - 1) / BR : 0;
+  // lse and D of the next tile's rows are loaded with it and stored a step later
+  float lse_r = INFINITY, dsum_r = 0.f;
+  int pos_r = 0, head_r = 0;
+  auto fetch = [&](int j) {
+    char* buf = smem + (j & 1) * 2 * TB;
+    const int r0 = start + j * BR, p0 = r0 / a.group;
+    const i32x4 rq = make_rsrc((const T*)a.q + (int64_t)(q0 + p0) * a.q_row + kvh * a.group * a.q_head);
+    const i32x4 rg = make_rsrc((const T*)a.dout + (int64_t)(q0 + p0) * a.g_row + kvh * a.group * a.g_head);
+    auto at = [&](int row, int64_t rs, int64_t hs) {
+      const int r = r0 + row, p = r / a.group, g = r - p * a.group;
+      return r < rows ? (p - p0) * (int)(rs * sizeof(T)) + g * (int)(hs * sizeof(T)) : -1;
+    };
+    stage<T, DP, BR>(rq, buf, a.dim, [&](int row) { return at(row, a.q_row, a.q_head); });
+    stage<T, DP, BR>(rg, buf + TB, a.dim, [&](int row) { return at(row, a.g_row, a.g_head); });
+    if (threadIdx.x < BR) {
+      const int r = r0 + threadIdx.x;
+      lse_r = INFINITY;   // a row past the end: p = 0
+      dsum_r = 0.f;
+      if (r < rows) {
+        const int p = r / a.group, g = r - p * a.group;
+        const int64_t x = (int64_t)(q0 + p) * heads + kvh * a.group + g;
+        lse_r = a.lse[x];
+        dsum_r = a.dsum[x];
+        pos_r = p;
+        head_r = g;
+      }
+    }
+  };
+  auto publish = [&](int j) {
+    if (threadIdx.x < BR) {
+      const int x = (j & 1) * BR + threadIdx.x;
+      lse_s[x] = lse_r;
+      dsum_s[x] = dsum_r;
+      if constexpr (BIAS) {
+        pos_s[x] = pos_r;
+        head_s[x] = head_r;
+      }
+    }
+  };
+
+  const float c = a.scale * LOG2E;
+  f32x16 dk[TL::ND], dv[TL::ND];
+#pragma unroll
+  for (int t = 0; t < TL::ND; ++t) dk[t] = dv[t] = zero16();
+
+  if (nt > 0) fetch(0);
+  for (int j = 0; j < nt; ++j) {
+    dpconv::wait_vmcnt<0>();
+    publish(j);
+    __syncthreads();
+    if (j + 1 < nt) fetch(j + 1);
+    const char* buf = smem + (j & 1) * 2 * TB;
+    const int r0 = start + j * BR;
+    if (first >= lk) continue;
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+      const int r32 = r0 + 32 * u;
+      if (r32 >= rows) break;
+      if (r32 + 31 < wfirst) continue;
+      const int x0 = (j & 1) * BR + 32 * u + 4 * h;
+      f32x16 s = rows_mma<T, DP>(buf, u, lane, kf);
+      if constexpr (BIAS) {
+        const int pf = r32 / a.group + off, pl = min(r32 + 31, rows - 1) / a.group + off;
+        const int one = bias.one_bucket(first - pl, first + 31 - pf);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int x = x0 + 8 * (i / 4) + (i & 3);
+          const int b = one >= 0 ? one : bias.bucket(key - pos_s[x] - off);
+          s[i] = fmaf(s[i], a.scale, bias.tab[head_s[x] * bias.nb + b]);
+        }
+      }
+      f32x16 p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + x0 + 8 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = s[4 * e + i];
+          p[4 * e + i] = __builtin_amdgcn_exp2f(BIAS ? (v - ls[i]) * LOG2E : fmaf(v, c, -ls[i]));
+        }
+      }
+      if (r32 < wlast || !ok) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (r32 + 8 * (i / 4) + 4 * h + (i & 3) < mine || !ok) p[i] = 0.f;
+      }
+      cols_mma<T, DP>(buf + TB, u, lane, p, dv);
+      const f32x16 dp = rows_mma<T, DP>(buf + TB, u, lane, vf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const f32x4 ds = *reinterpret_cast<const f32x4*>(dsum_s + x0 + 8 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[4 * e + i] *= dp[4 * e + i] - ds[i];
+      }
+      cols_mma<T, DP>(buf, u, lane, p, dk);
+    }
+  }
+
+  if (ok) {
+    const int64_t at = ((int64_t)(k0 + key) * a.hkv + kvh) * a.dim;
+#pragma unroll
+    for (int t = 0; t < TL::ND; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 32 * t + 8 * e + 4 * h;
+        if (d < a.dim) {
+          typedef T T4 __attribute__((ext_vector_type(4)));
+          T4 x, y;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = from_f32<T>(dk[t][4 * e + i] * a.scale);
+            y[i] = from_f32<T>(dv[t][4 * e + i]);
+          }
+          *reinterpret_cast<T4*>((T*)a.dk + at + d) = x;
+          *reinterpret_cast<T4*>((T*)a.dv + at + d) = y;
+        }
+      }
+  }
+}
+
+static int grow_lds(const void* kern, int lds) {
+  if (lds <= 65536) return 0;
+  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  DP_REQUIRE(e == hipSuccess, "dp_packed_attn_bwd: %d bytes of LDS: %s", lds, hipGetErrorString(e));
+  return 0;
+}
+
+template <typename T, int DP, bool BIAS>
+int launch(const Args& a, void* dbias, int bias_f32, hipStream_t s) {
+  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  if (a.tq > 0) {
+    const int lds = 4 * BN * Tile<T, DP>::RB + (BIAS ? a.buckets * NT * 4 + bias_lds(a) : 0);
+    const auto kern = packed_bwd_q_kernel<T, DP, BN, BIAS>;
+    if (const int rc = grow_lds((const void*)kern, lds)) return rc;
+    hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a);
+  }
+  if (a.tk > 0) {
+    const int lds = 4 * BN * Tile<T, DP>::RB + 16 * BN * 2 + bias_lds(a);
+    const auto kern = packed_bwd_kv_kernel<T, DP, BN, BIAS>;
+    if (const int rc = grow_lds((const void*)kern, lds)) return rc;
+    const int tiles = a.tk / BM + a.nseq + 1;
+    hipLaunchKernelGGL(kern, dim3(tiles * a.hkv), dim3(NT), lds, s, a);
+  }
+  if constexpr (BIAS) {
+    const int tiles = a.tq > 0 ? a.tiles : 0;
+    if (bias_f32)
+      hipLaunchKernelGGL((packed_dbias_kernel<float>), dim3(a.hkv * a.group), dim3(NT), 0, s, (float*)dbias,
+                         a.dbias_part, tiles, a.hkv, a.group, a.buckets);
+    else
+      hipLaunchKernelGGL((packed_dbias_kernel<T>), dim3(a.hkv * a.group), dim3(NT), 0, s, (T*)dbias, a.dbias_part,
+                         tiles, a.hkv, a.group, a.buckets);
+  }
+  return dp_check_launch("dp_packed_attn_bwd");
+}
+
+template <typename T, bool BIAS>
+int launch_dim(const Args& a, void* dbias, int bias_f32, hipStream_t s) {
+  if (a.dim <= 32) return launch<T, 32, BIAS>(a, dbias, bias_f32, s);
+  if (a.dim <= 64) return launch<T, 64, BIAS>(a, dbias, bias_f32, s);
+  return launch<T, 128, BIAS>(a, dbias, bias_f32, s);
+}
+
+}  // namespace
+
+extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
+  Args a;
+  if (const int rc = dp_packed_attn_args(d, &a, "dp_packed_attn_bwd", true)) return rc;
+  DP_REQUIRE((d->lse && d->dout && d->dq) || d->tq == 0, "dp_packed_attn_bwd: no lse, dout or dq");
+  DP_REQUIRE((d->dk && d->dv) || d->tk == 0, "dp_packed_attn_bwd: no dk or dv");
+  DP_REQUIRE(!d->bias || d->dbias, "dp_packed_attn_bwd: no dbias");
+  DP_REQUIRE(((uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0,
+             "dp_packed_attn_bwd: gradients are not 16-byte aligned");
+  const int64_t need = dp_packed_attn_ws_bytes(d, 1);
+  DP_REQUIRE(d->ws_bytes >= need && (d->ws || !need), "dp_packed_attn_bwd: workspace holds %lld bytes, needs %lld",
+             (long long)d->ws_bytes, (long long)need);
+  a.dout = d->dout; a.g_row = d->g_row; a.g_head = d->g_head; a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+  a.dsum = (float*)d->ws;
+  a.dbias_part = a.dsum + (int64_t)d->tq * d->heads;
+  hipStream_t s = as_stream(stream);
+  const int bf = d->bias_dtype == DP_F32;
+  if (d->dtype == DP_BF16)
+    return a.bias ? launch_dim<bf16_t, true>(a, d->dbias, bf, s) : launch_dim<bf16_t, false>(a, d->dbias, bf, s);
+  return a.bias ? launch_dim<float, true>(a, d->dbias, bf, s) : launch_dim<float, false>(a, d->dbias, bf, s);
+}

@@ -737,6 +737,45 @@ int dp_maxpool2x2_pad_rb_bwd(const void* x, int64_t x_bstride, int32_t x_pstride
 /* ---- Token sequences and gradients of separate tensors. Callers: detrpose_amd/{attention,norm,
  * gradients}.py. */
 
+/* Attention over packed sequences: sequence b owns query rows [cu_q[b], cu_q[b + 1]) of q / out and key
+ * rows [cu_k[b], cu_k[b + 1]) of k / v (cu_*: device int32 [nseq + 1], rising, the first taken as 0;
+ * values past tq / tk are cut there). Query i of lq has position i + lk - lq (the last query sits on the
+ * last key); causal: it sees keys j <= position. s = scale q.k (+ bias), p = softmax over the seen
+ * keys (a query that sees none: zeros), out = p v. Query head h reads key head h / (heads / kv_heads).
+ *  q, out [tq][heads][dim], k, v [tk][kv_heads][dim] of dtype, element strides *_row / *_head, dim
+ *  contiguous, every row 16-byte aligned; dim a multiple of 8 up to 128.
+ *  lse: f32 [tq][heads] (the log of the softmax's denominator, in the backward's units), or NULL.
+ *  bias: NULL or a learned table [buckets][heads] (f32, or dtype): the bias of pair (i, j) is
+ *  bias[bucket(j - position)][h]. n = |j - position| (one direction: max(position - j, 0)) falls into
+ *  the bucket numbered by how many of edge[0 .. nb - 2] are <= n, nb = buckets (both directions: half of
+ *  them, and keys behind the query's position take the other half). edge: from 1, not falling, the last <= 4096.
+ *  fill_tail: rows of out behind the last sequence are written as zeros (else left as they are).
+ *  ws: dp_packed_attn_ws_bytes(desc, 0) bytes. */
+typedef struct dp_packed_attn {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+  const int32_t *cu_q, *cu_k;
+  int32_t nseq, tq, tk, heads, kv_heads, dim, causal, fill_tail;
+  float scale;
+  int32_t dtype;
+  const void* bias;
+  int32_t bias_dtype, buckets, both;
+  int32_t edge[64];
+  void* ws;
+  int64_t ws_bytes;
+  /* backward only: dout strided like o_* under its own strides; dq [tq][heads][dim], dk, dv
+   * [tk][kv_heads][dim] contiguous of dtype, written whole (rows behind the last sequence as zeros);
+   * dbias [buckets][heads] of bias_dtype. Deterministic: no atomics. ws: dp_packed_attn_ws_bytes(desc, 1). */
+  const void* dout;
+  int64_t g_row, g_head;
+  void *dq, *dk, *dv, *dbias;
+} dp_packed_attn;
+int64_t dp_packed_attn_ws_bytes(const dp_packed_attn* d, int32_t backward);
+int dp_packed_attn_fwd(const dp_packed_attn* d, void* stream);
+int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream);
+
 /* Root-mean-square norm over rows of c elements: r = x (+ res, rounded to dtype and written when r is
  * not NULL), rstd = 1 / sqrt(mean r^2 + eps) (f32 [rows], written when not NULL), y = r rstd weight.
  * x / res rows ld_x / ld_res apart, y / r contiguous; weight [c] f32 or dtype. c up to 8192 (f32),
