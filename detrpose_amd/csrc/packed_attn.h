@@ -47,6 +47,10 @@ struct Args {
   const int32_t *cu_q, *cu_k;
   int nseq, tq, tk, hkv, group, dim, causal, tiles;
   float scale;
+  // split keys (forward): key chunk at least, most chunks of one sequence, and where the parts go
+  int chunk, splits;
+  float *part, *part_lse;
+  int* part_n;
   // bias
   const void* bias;
   int bias_f32, buckets, both, nedge;
@@ -57,6 +61,9 @@ struct Args {
   void *dq, *dk, *dv;
   float* dsum;
   float* dbias_part;
+  int ktiles, cut_rows, cuts;   // dk / dv: blocks, rows of a cut at least, most cuts of one sequence
+  float* kv_part;
+  int* kv_n;
 };
 
 template <typename T> struct Tr;
@@ -202,12 +209,13 @@ __device__ __forceinline__ void tile_barrier() {
 // The lengths are on the device only: a launch has as many blocks as the packed total allows at
 // most, and every wave finds its block's (sequence, tile) by a scan over the sequences, 64 at a time.
 // nseq counts one more when the rows behind the last sequence are an item of their own (tail).
-struct Item { int b, tile, start, len; };
+struct Item { int b, sub, start, len; };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// rows_of(len) rows of `per` a tile
-__device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total, int mult, int per, bool tail, int idx,
+// cu's sequences, sequence b counting items(b, its length) blocks; it.sub: which of them idx is
+template <typename COUNT>
+__device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total, bool tail, int idx, COUNT items,
                                           Item& it) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -219,7 +227,7 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total
       start = b ? clampi(cu[b], 0, total) : 0;
       len = max(0, (b < nseq ? clampi(cu[b + 1], 0, total) : total) - start);
     }
-    const int cnt = (len * mult + per - 1) / per;
+    const int cnt = len ? items(b, len) : 0;
     int inc = cnt;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -231,7 +239,7 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total
       const unsigned long long m = __ballot(idx < before + inc);
       const int l = __ffsll((long long)m) - 1;
       it.b = __builtin_amdgcn_readfirstlane(base + l);
-      it.tile = __builtin_amdgcn_readfirstlane(idx - before - __shfl(inc - cnt, l, 64));
+      it.sub = __builtin_amdgcn_readfirstlane(idx - before - __shfl(inc - cnt, l, 64));
       it.start = __builtin_amdgcn_readfirstlane(__shfl(start, l, 64));
       it.len = __builtin_amdgcn_readfirstlane(__shfl(len, l, 64));
       return true;
@@ -242,9 +250,14 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total
 }
 
 // start and length of sequence b (nothing for the tail)
+__device__ __forceinline__ int2 seq_at(const int32_t* cu, int nseq, int total, int b) {
+  const int start = b && b < nseq ? clampi(cu[b], 0, total) : 0;
+  return int2{start, b < nseq ? max(0, clampi(cu[b + 1], 0, total) - start) : 0};
+}
 __device__ __forceinline__ void seq_of(const int32_t* cu, int nseq, int total, int b, int& start, int& len) {
-  start = b && b < nseq ? clampi(cu[b], 0, total) : 0;
-  len = b < nseq ? max(0, clampi(cu[b + 1], 0, total) - start) : 0;
+  const int2 s = seq_at(cu, nseq, total, b);
+  start = s.x;
+  len = s.y;
   start = __builtin_amdgcn_readfirstlane(start);
   len = __builtin_amdgcn_readfirstlane(len);
 }

@@ -14,23 +14,27 @@
 // per tile where the whole tile lies in one bucket); the block then adds the bins of a head's rows and
 // writes one part per block, and packed_dbias_kernel adds the parts, all in fixed orders.
 #include "packed_attn.h"
+#include <algorithm>
 
 int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what, bool backward);
 
 namespace {
 using namespace dppa;
 
-template <typename T, int DP, int BN, bool BIAS>
-__global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
+// WK waves of a block share its rows and take the key tile's subtiles in turn, as in the forward
+template <typename T, int DP, int WK, int BN, bool BIAS>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_bwd_q_kernel(const Args a) {
   using TL = Tile<T, DP>;
-  constexpr int TB = BN * TL::RB, NS = BN / 32;
+  constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
+  static_assert(WK == 1 || 4 * TB >= 4 * 32 * OP * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int wk = wave % WK, wr = wave / WK;
   const int kvh = blockIdx.x % a.hkv, tile = a.tiles - 1 - blockIdx.x / a.hkv;
   const int heads = a.hkv * a.group;
   float* part = BIAS ? a.dbias_part + ((int64_t)tile * a.hkv + kvh) * a.group * a.buckets : nullptr;
   Item it;
-  if (!find_item(a.cu_q, a.nseq, a.tq, a.group, BM, true, tile, it)) {
+  if (!find_item(a.cu_q, a.nseq, a.tq, true, tile, [&](int, int len) { return (len * a.group + ROWS - 1) / ROWS; }, it)) {
     if constexpr (BIAS)
       for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) part[i] = 0.f;
     return;
@@ -38,15 +42,15 @@ __global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
   const int q0 = it.start, lq = it.len;
   int k0, lk;
   seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
-  const int off = lk - lq, rows = lq * a.group, row0 = it.tile * BM;
-  const int first = row0 + 32 * wave, r = first + (lane & 31);
+  const int off = lk - lq, rows = lq * a.group, row0 = it.sub * ROWS;
+  const int first = row0 + 32 * wr, r = first + (lane & 31);
   const bool ok = r < rows;
   const int rc = min(r, rows - 1), pos = rc / a.group, g = rc - pos * a.group, head = kvh * a.group + g;
   auto limit = [&](int row) {
     return a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
   };
   const int lim = limit(r), wmin = limit(first), wmax = first < rows ? limit(first + 31) : 0;
-  const int nt = (limit(row0 + BM - 1) + BN - 1) / BN;
+  const int nt = (limit(row0 + ROWS - 1) + BN - 1) / BN;
   Bias bias{};
   float* bins = nullptr;
   if constexpr (BIAS) {
@@ -73,7 +77,7 @@ __global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
     }
     D = half_sum(D);
   }
-  if (ok && h == 0) a.dsum[at] = D;
+  if (ok && h == 0 && wk == 0) a.dsum[at] = D;
   const float lse = ok ? a.lse[at] : INFINITY;
 
   auto fetch = [&](int j) {
@@ -100,8 +104,8 @@ __global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
     const int key0 = j * BN;
     if (key0 >= wmax) continue;
 #pragma unroll
-    for (int u = 0; u < NS; ++u) {
-      const int k32 = key0 + 32 * u;
+    for (int un = 0; un < NS; ++un) {
+      const int u = NS * wk + un, k32 = key0 + 32 * u;
       if (k32 >= wmax) break;
       f32x16 s = rows_mma<T, DP>(buf, u, lane, qf);
       const f32x16 dp = rows_mma<T, DP>(buf + TB, u, lane, gf);
@@ -147,21 +151,49 @@ __global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
     }
   }
 
-  if (ok) {
-    T* op = (T*)a.dq + at * a.dim;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  if constexpr (WK == 1) {
+    if (ok) {
+#pragma unroll
+      for (int t = 0; t < TL::ND; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 32 * t + 8 * e + 4 * h;
+          if (d < a.dim) {
+            T4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(dq[t][4 * e + i] * a.scale);
+            *reinterpret_cast<T4*>((T*)a.dq + at * a.dim + d) = w;
+          }
+        }
+    }
+  } else {
+    __syncthreads();
+    float* oo = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int t = 0; t < TL::ND; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 32 * t + 8 * e + 4 * h;
-        if (d < a.dim) {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 w;
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(oo + (wave * 32 + (lane & 31)) * OP + 32 * t + 8 * e + 4 * h) =
+            f32x4{dq[t][4 * e], dq[t][4 * e + 1], dq[t][4 * e + 2], dq[t][4 * e + 3]};
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * (DP / 4); i += NT) {
+      const int jr = i / (DP / 4), d = (i - jr * (DP / 4)) * 4, row = row0 + jr;
+      if (row >= rows || d >= a.dim) continue;
+      const int w0 = (jr >> 5) * WK * 32 + (jr & 31), rp = row / a.group;
+      f32x4 sum = *reinterpret_cast<const f32x4*>(oo + w0 * OP + d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(dq[t][4 * e + i] * a.scale);
-          *reinterpret_cast<T4*>(op + d) = w;
-        }
+      for (int w = 1; w < WK; ++w) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(oo + (w0 + 32 * w) * OP + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
       }
+      T4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(sum[e] * a.scale);
+      const int64_t x = (int64_t)(q0 + rp) * heads + kvh * a.group + row - rp * a.group;
+      *reinterpret_cast<T4*>((T*)a.dq + x * a.dim + d) = w;
+    }
   }
   if constexpr (BIAS) {
     __syncthreads();
@@ -170,10 +202,12 @@ __global__ __launch_bounds__(NT, 2) void packed_bwd_q_kernel(const Args a) {
       const int pg = p / a.buckets, b = p - pg * a.buckets;
       int rr = (pg - row0 % a.group + a.group) % a.group;   // the block's first row of this head
       float t = 0.f;
-      for (; rr < min(BM, rows - row0); rr += a.group) {
-        const float* x = all + b * NT + (rr >> 5) * 64 + (rr & 31);
-        t += x[0] + x[32];
-      }
+      for (; rr < min(ROWS, rows - row0); rr += a.group)
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float* x = all + b * NT + ((rr >> 5) * WK + w) * 64 + (rr & 31);
+          t += x[0] + x[32];
+        }
       part[p] = t;
     }
   }
@@ -196,6 +230,12 @@ __global__ __launch_bounds__(NT) void packed_dbias_kernel(TB* __restrict__ out, 
     out[(int64_t)b * hkv * group + head] = from_f32<TB>((sm[b] + sm[64 + b]) + (sm[128 + b] + sm[192 + b]));
 }
 
+// rows [cut * step, ...) of a sequence's cuts
+__device__ __forceinline__ int cuts_of(const Args& a, int rows) {
+  return a.cuts <= 1 ? 1 : clampi((rows + a.cut_rows - 1) / a.cut_rows, 1, a.cuts);
+}
+__device__ __forceinline__ int cut_step(int rows, int cuts) { return ((rows + cuts - 1) / cuts + 31) / 32 * 32; }
+
 template <typename T, int DP, int BR, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kernel(const Args a) {
   using TL = Tile<T, DP>;
@@ -209,17 +249,27 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int kvh = blockIdx.x % a.hkv;
   const int heads = a.hkv * a.group;
+  auto tiles_of = [&](int len) { return (len + BM - 1) / BM; };
   Item it;
-  if (!find_item(a.cu_k, a.nseq, a.tk, 1, BM, true, blockIdx.x / a.hkv, it)) return;
+  if (!find_item(a.cu_k, a.nseq, a.tk, true, blockIdx.x / a.hkv,
+                 [&](int b, int len) {
+                   return tiles_of(len) * cuts_of(a, seq_at(a.cu_q, a.nseq, a.tq, b).y * a.group);
+                 }, it))
+    return;
   const int k0 = it.start, lk = it.len;
   int q0, lq;
   seq_of(a.cu_q, a.nseq, a.tq, it.b, q0, lq);
-  const int off = lk - lq, rows = lq * a.group;
-  const int first = it.tile * BM + 32 * wave, key = first + (lane & 31);
+  const int off = lk - lq, rows = lq * a.group, ntile = tiles_of(lk);
+  const int cuts = cuts_of(a, rows), cut = it.sub / ntile, tile = it.sub - cut * ntile;
+  const int first = tile * BM + 32 * wave, key = first + (lane & 31);
   const bool ok = key < lk;
   // the first row that sees a key
   auto sees = [&](int kk) { return a.causal ? max(0, kk - off) * a.group : 0; };
   const int mine = sees(key), wfirst = sees(first), wlast = sees(min(first + 31, lk - 1));
+  // this block's rows [start, end)
+  const int seen = sees(tile * BM) / 32 * 32, step = cuts > 1 ? cut_step(rows, cuts) : 0;
+  const int start = max(seen, cut * step), end = cuts > 1 ? min(rows, (cut + 1) * step) : rows;
+  if (start >= end && cuts > 1) return;
   Bias bias{};
   if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB + 16 * BR * 2, kvh);
 
@@ -227,32 +277,38 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   load_frags<T, DP>((const T*)a.k + (int64_t)(k0 + min(key, lk - 1)) * a.k_row + kvh * a.k_head, ok, a.dim, h, kf);
   load_frags<T, DP>((const T*)a.v + (int64_t)(k0 + min(key, lk - 1)) * a.v_row + kvh * a.v_head, ok, a.dim, h, vf);
 
-  const int start = sees(it.tile * BM) / 32 * 32;
-  const int nt = rows > start ? (rows - start + BR - 1) / BR : 0;
+  const int nt = end > start ? (end - start + BR - 1) / BR : 0;
+  const float invg = 1.f / (float)a.group;
   // lse and D of the next tile's rows are loaded with it and stored a step later
   float lse_r = INFINITY, dsum_r = 0.f;
   int pos_r = 0, head_r = 0;
   auto fetch = [&](int j) {
     char* buf = smem + (j & 1) * 2 * TB;
-    const int r0 = start + j * BR, p0 = r0 / a.group;
+    const int r0 = start + j * BR, p0 = r0 / a.group, skip = r0 - p0 * a.group;
     const i32x4 rq = make_rsrc((const T*)a.q + (int64_t)(q0 + p0) * a.q_row + kvh * a.group * a.q_head);
     const i32x4 rg = make_rsrc((const T*)a.dout + (int64_t)(q0 + p0) * a.g_row + kvh * a.group * a.g_head);
+    // (query, head) of the tile's row: a small quotient, exact in f32
+    auto split = [&](int row, int& p, int& g) {
+      p = (int)(((float)(skip + row) + 0.5f) * invg);
+      g = skip + row - p * a.group;
+    };
     auto at = [&](int row, int64_t rs, int64_t hs) {
-      const int r = r0 + row, p = r / a.group, g = r - p * a.group;
-      return r < rows ? (p - p0) * (int)(rs * sizeof(T)) + g * (int)(hs * sizeof(T)) : -1;
+      int p, g;
+      split(row, p, g);
+      return r0 + row < end ? p * (int)(rs * sizeof(T)) + g * (int)(hs * sizeof(T)) : -1;
     };
     stage<T, DP, BR>(rq, buf, a.dim, [&](int row) { return at(row, a.q_row, a.q_head); });
     stage<T, DP, BR>(rg, buf + TB, a.dim, [&](int row) { return at(row, a.g_row, a.g_head); });
     if (threadIdx.x < BR) {
-      const int r = r0 + threadIdx.x;
       lse_r = INFINITY;   // a row past the end: p = 0
       dsum_r = 0.f;
-      if (r < rows) {
-        const int p = r / a.group, g = r - p * a.group;
-        const int64_t x = (int64_t)(q0 + p) * heads + kvh * a.group + g;
+      if (r0 + (int)threadIdx.x < end) {
+        int p, g;
+        split(threadIdx.x, p, g);
+        const int64_t x = (int64_t)(q0 + p0 + p) * heads + kvh * a.group + g;
         lse_r = a.lse[x];
         dsum_r = a.dsum[x];
-        pos_r = p;
+        pos_r = p0 + p;
         head_r = g;
       }
     }
@@ -286,7 +342,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
       const int r32 = r0 + 32 * u;
-      if (r32 >= rows) break;
+      if (r32 >= end) break;
       if (r32 + 31 < wfirst) continue;
       const int x0 = (j & 1) * BR + 32 * u + 4 * h;
       f32x16 s = rows_mma<T, DP>(buf, u, lane, kf);
@@ -328,25 +384,99 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   }
 
   if (ok) {
-    const int64_t at = ((int64_t)(k0 + key) * a.hkv + kvh) * a.dim;
+    const int64_t kr = (int64_t)(k0 + key) * a.hkv + kvh;
+    float* part = a.kv_part + ((int64_t)cut * a.tk * a.hkv + kr) * 2 * a.dim;
 #pragma unroll
     for (int t = 0; t < TL::ND; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = 32 * t + 8 * e + 4 * h;
         if (d < a.dim) {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 x, y;
+          f32x4 x, y;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = from_f32<T>(dk[t][4 * e + i] * a.scale);
-            y[i] = from_f32<T>(dv[t][4 * e + i]);
+            x[i] = dk[t][4 * e + i] * a.scale;
+            y[i] = dv[t][4 * e + i];
           }
-          *reinterpret_cast<T4*>((T*)a.dk + at + d) = x;
-          *reinterpret_cast<T4*>((T*)a.dv + at + d) = y;
+          if (cuts > 1) {
+            *reinterpret_cast<f32x4*>(part + d) = x;
+            *reinterpret_cast<f32x4*>(part + a.dim + d) = y;
+          } else {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            T4 u, w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              u[i] = from_f32<T>(x[i]);
+              w[i] = from_f32<T>(y[i]);
+            }
+            *reinterpret_cast<T4*>((T*)a.dk + kr * a.dim + d) = u;
+            *reinterpret_cast<T4*>((T*)a.dv + kr * a.dim + d) = w;
+          }
         }
       }
+    // the last cut's rows see every key: it says which cuts there are (and 0 of them where it wrote the result)
+    if (a.cuts > 1 && cut == cuts - 1 && h == 0) a.kv_n[kr] = cuts > 1 ? (seen / step) << 16 | cuts : 0;
   }
+}
+
+// keys whose rows were cut: dk and dv = the sums of the parts in the order of the cuts, four elements a thread
+template <typename T, int DP>
+__global__ __launch_bounds__(NT) void packed_kv_join_kernel(const Args a) {
+  constexpr int TPR = DP / 4;
+  const int64_t all = (int64_t)a.tk * a.hkv;
+  const int64_t kr = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const int d = (threadIdx.x % TPR) * 4;
+  if (kr >= all || d >= a.dim) return;
+  const int n = a.kv_n[kr], from = n >> 16, to = min(n & 0xffff, a.cuts);
+  if (n <= 0) return;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll 4
+  for (int c = from; c < to; ++c) {
+    const float* part = a.kv_part + (c * all + kr) * 2 * a.dim + d;
+    const f32x4 u = *reinterpret_cast<const f32x4*>(part), w = *reinterpret_cast<const f32x4*>(part + a.dim);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] += u[i];
+      y[i] += w[i];
+    }
+  }
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 u, w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u[i] = from_f32<T>(x[i]);
+    w[i] = from_f32<T>(y[i]);
+  }
+  *reinterpret_cast<T4*>((T*)a.dk + kr * a.dim + d) = u;
+  *reinterpret_cast<T4*>((T*)a.dv + kr * a.dim + d) = w;
+}
+
+// How the two kernels are cut. Lengths are on the device, so the rule goes by totals.
+struct Plan { int wk, items, cut_rows, cuts, ktiles; };
+static Plan plan_of(const dp_packed_attn* d) {
+  const int64_t group = d->heads / d->kv_heads, rows = d->tq * group, seqs = std::max(1, d->nseq);
+  Plan p{1, 0, 0, 1, 0};
+  const int64_t wide = (rows / BM + 1) * d->kv_heads;
+  if (wide < 256 && d->tk <= 2048 * seqs) p.wk = d->dtype == DP_F32 && d->dim > 64 ? 2 : 4;
+  // the bins beside the waves' larger key tile: where both do not fit the LDS, the waves lie along the rows
+  const int dp = d->dim <= 32 ? 32 : d->dim <= 64 ? 64 : 128, last = d->bias && d->buckets > 2 ? 4096 + 16 : 16;
+  if (d->bias && 4 * 32 * p.wk * dp * (d->dtype == DP_F32 ? 4 : 2) + d->buckets * (NT + (int)group) * 4 + last > 163840) p.wk = 1;
+  p.items = (int)(rows / (BM / p.wk) + d->nseq + 1);
+  // a block of keys walks all rows that see them: the longest such walk bounds the time unless it is
+  // cut. About 1024 blocks (causal order leaves half of the cuts empty), at least 512 rows each
+  const int64_t kblocks = (int64_t)(d->tk / BM + 1) * d->kv_heads;
+  int64_t cuts = std::min<int64_t>(16, (1024 + kblocks - 1) / kblocks * (d->causal ? 2 : 1));
+  cuts = std::min(cuts, std::max<int64_t>(1, ((int64_t)1 << 30) / std::max<int64_t>(1, (int64_t)d->tk * d->kv_heads * d->dim * 8)));
+  const int64_t per = std::max<int64_t>(512, ((rows + cuts - 1) / cuts + 63) / 64 * 64);
+  cuts = std::min(cuts, (rows + per - 1) / per);
+  int64_t tiles = d->tk / BM + d->nseq + 1;
+  if (cuts > 1) {
+    p.cuts = (int)cuts;
+    p.cut_rows = (int)per;
+    tiles = std::min(tiles * cuts, tiles + (d->tk / BM + 1) * (rows / per + 1));
+  }
+  p.ktiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+  return p;
 }
 
 static int grow_lds(const void* kern, int lds) {
@@ -356,21 +486,31 @@ static int grow_lds(const void* kern, int lds) {
   return 0;
 }
 
+template <typename T, int DP, int WK, bool BIAS>
+int launch_q(const Args& a, hipStream_t s) {
+  constexpr int BN = WK > 1 ? 32 * WK : sizeof(T) == 2 ? 64 : 32;
+  const int lds = 4 * BN * Tile<T, DP>::RB + (BIAS ? a.buckets * NT * 4 + bias_lds(a) : 0);
+  const auto kern = packed_bwd_q_kernel<T, DP, WK, BN, BIAS>;
+  if (const int rc = grow_lds((const void*)kern, lds)) return rc;
+  hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a);
+  return 0;
+}
+
 template <typename T, int DP, bool BIAS>
-int launch(const Args& a, void* dbias, int bias_f32, hipStream_t s) {
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
-  if (a.tq > 0) {
-    const int lds = 4 * BN * Tile<T, DP>::RB + (BIAS ? a.buckets * NT * 4 + bias_lds(a) : 0);
-    const auto kern = packed_bwd_q_kernel<T, DP, BN, BIAS>;
-    if (const int rc = grow_lds((const void*)kern, lds)) return rc;
-    hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a);
-  }
+int launch(const Args& a, int wk, void* dbias, int bias_f32, hipStream_t s) {
+  constexpr int BR = sizeof(T) == 2 ? 64 : 32;
+  constexpr int W = sizeof(T) == 2 || DP <= 64 ? 4 : 2;
+  if (a.tq > 0)
+    if (const int rc = wk > 1 ? launch_q<T, DP, W, BIAS>(a, s) : launch_q<T, DP, 1, BIAS>(a, s)) return rc;
   if (a.tk > 0) {
-    const int lds = 4 * BN * Tile<T, DP>::RB + 16 * BN * 2 + bias_lds(a);
-    const auto kern = packed_bwd_kv_kernel<T, DP, BN, BIAS>;
+    const int lds = 4 * BR * Tile<T, DP>::RB + 16 * BR * 2 + bias_lds(a);
+    const auto kern = packed_bwd_kv_kernel<T, DP, BR, BIAS>;
     if (const int rc = grow_lds((const void*)kern, lds)) return rc;
-    const int tiles = a.tk / BM + a.nseq + 1;
-    hipLaunchKernelGGL(kern, dim3(tiles * a.hkv), dim3(NT), lds, s, a);
+    hipLaunchKernelGGL(kern, dim3(a.ktiles * a.hkv), dim3(NT), lds, s, a);
+    if (a.cuts > 1) {
+      const int64_t n = (int64_t)a.tk * a.hkv, per = NT / (DP / 4);
+      hipLaunchKernelGGL((packed_kv_join_kernel<T, DP>), dim3((unsigned)((n + per - 1) / per)), dim3(NT), 0, s, a);
+    }
   }
   if constexpr (BIAS) {
     const int tiles = a.tq > 0 ? a.tiles : 0;
@@ -385,13 +525,21 @@ int launch(const Args& a, void* dbias, int bias_f32, hipStream_t s) {
 }
 
 template <typename T, bool BIAS>
-int launch_dim(const Args& a, void* dbias, int bias_f32, hipStream_t s) {
-  if (a.dim <= 32) return launch<T, 32, BIAS>(a, dbias, bias_f32, s);
-  if (a.dim <= 64) return launch<T, 64, BIAS>(a, dbias, bias_f32, s);
-  return launch<T, 128, BIAS>(a, dbias, bias_f32, s);
+int launch_dim(const Args& a, int wk, void* dbias, int bias_f32, hipStream_t s) {
+  if (a.dim <= 32) return launch<T, 32, BIAS>(a, wk, dbias, bias_f32, s);
+  if (a.dim <= 64) return launch<T, 64, BIAS>(a, wk, dbias, bias_f32, s);
+  return launch<T, 128, BIAS>(a, wk, dbias, bias_f32, s);
 }
 
 }  // namespace
+
+int64_t dp_packed_bwd_ws_bytes(const dp_packed_attn* d) {
+  const Plan p = plan_of(d);
+  int64_t n = (int64_t)d->tq * d->heads + (d->bias ? (int64_t)p.items * d->heads * d->buckets : 0);
+  n = (n + 3) / 4 * 4;
+  if (p.cuts > 1) n += (int64_t)d->tk * d->kv_heads * ((int64_t)p.cuts * 2 * d->dim + 1);
+  return n * 4;
+}
 
 extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
   Args a;
@@ -405,11 +553,19 @@ extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
   DP_REQUIRE(d->ws_bytes >= need && (d->ws || !need), "dp_packed_attn_bwd: workspace holds %lld bytes, needs %lld",
              (long long)d->ws_bytes, (long long)need);
   a.dout = d->dout; a.g_row = d->g_row; a.g_head = d->g_head; a.dq = d->dq; a.dk = d->dk; a.dv = d->dv;
+  const Plan p = plan_of(d);
+  a.tiles = p.items;
+  a.ktiles = p.ktiles;
+  a.cuts = p.cuts;
+  a.cut_rows = p.cut_rows;
+  DP_REQUIRE((int64_t)p.ktiles * a.hkv < INT32_MAX, "dp_packed_attn_bwd: too many tiles");
   a.dsum = (float*)d->ws;
   a.dbias_part = a.dsum + (int64_t)d->tq * d->heads;
+  a.kv_part = a.dsum + ((int64_t)d->tq * d->heads + (a.bias ? (int64_t)p.items * d->heads * d->buckets : 0) + 3) / 4 * 4;
+  a.kv_n = (int*)(a.kv_part + (int64_t)p.cuts * a.tk * a.hkv * 2 * a.dim);
   hipStream_t s = as_stream(stream);
   const int bf = d->bias_dtype == DP_F32;
   if (d->dtype == DP_BF16)
-    return a.bias ? launch_dim<bf16_t, true>(a, d->dbias, bf, s) : launch_dim<bf16_t, false>(a, d->dbias, bf, s);
-  return a.bias ? launch_dim<float, true>(a, d->dbias, bf, s) : launch_dim<float, false>(a, d->dbias, bf, s);
+    return a.bias ? launch_dim<bf16_t, true>(a, p.wk, d->dbias, bf, s) : launch_dim<bf16_t, false>(a, p.wk, d->dbias, bf, s);
+  return a.bias ? launch_dim<float, true>(a, p.wk, d->dbias, bf, s) : launch_dim<float, false>(a, p.wk, d->dbias, bf, s);
 }

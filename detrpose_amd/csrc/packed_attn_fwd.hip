@@ -17,9 +17,8 @@ constexpr float GROW = 8.f;   // log2 of how far p may pass 1 before m moves
 
 // A row again, key by key: only for a wave whose result holds a NaN. In the products a hidden key's
 // weight is 0, but 0 x inf or NaN (a value that causal order hides) is NaN: here hidden keys are not read.
-template <typename T, bool BIAS>
-__device__ __forceinline__ void slow_row(const Args& a, const Bias& bias, int kvh, int g, int pos, int q0, int k0, int lk,
-                                      int lim, int off) {
+template <typename T, typename BIASOF>
+__device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos, int q0, int k0, int lim, BIASOF bias) {
   const int lane = threadIdx.x & 63;
   const int head = kvh * a.group + g;
   const T* q = (const T*)a.q + (int64_t)(q0 + pos) * a.q_row + head * a.q_head;
@@ -27,9 +26,7 @@ __device__ __forceinline__ void slow_row(const Args& a, const Bias& bias, int kv
     const T* k = (const T*)a.k + (int64_t)(k0 + j) * a.k_row + kvh * a.k_head;
     float s = 0.f;
     for (int d = 0; d < a.dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-    s *= a.scale;
-    if constexpr (BIAS) s += bias.tab[g * bias.nb + bias.bucket(j - pos - off)];
-    return s;
+    return s * a.scale + bias(j);
   };
   float m = -INFINITY;
   for (int j = lane; j < lim; j += 64) m = fmaxf(m, score(j));
@@ -53,29 +50,46 @@ __device__ __forceinline__ void slow_row(const Args& a, const Bias& bias, int kv
   if (lane + 64 < a.dim) o[lane + 64] = from_f32<T>(o1 * inv);
 }
 
-template <typename T, int DP, int BN, bool BIAS>
-__global__ __launch_bounds__(NT, 2) void packed_fwd_kernel(const Args a, int fill_tail) {
+// chunks that a sequence's keys are cut into, for a tile of `rows` rows
+__device__ __forceinline__ int splits_of(const Args& a, int lk, int rows) {
+  return a.splits <= 1 ? 1 : clampi((lk + a.chunk - 1) / max(a.chunk, 16 * rows), 1, a.splits);
+}
+
+// WK waves of a block share its rows and walk the key tile's subtiles in turn; 4 / WK of them, 32 rows
+// each, lie along the rows.
+template <typename T, int DP, int WK, int BN, bool BIAS>
+__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_fwd_kernel(const Args a, int fill_tail) {
   using TL = Tile<T, DP>;
-  constexpr int TB = BN * TL::RB, NS = BN / 32;
+  constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
+  static_assert(WK == 1 || 4 * TB >= (4 * 32 * (OP + 2) + 2 * ROWS) * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int wk = wave % WK, wr = wave / WK;
   const int kvh = blockIdx.x % a.hkv;
+  auto tiles_of = [&](int len) { return (len * a.group + ROWS - 1) / ROWS; };
+  auto cuts_of = [&](int lq, int lk) { return splits_of(a, lk, min(ROWS, lq * a.group)); };
   Item it;
   // the last tiles first: in causal order they have the most keys
-  if (!find_item(a.cu_q, a.nseq, a.tq, a.group, BM, fill_tail, a.tiles - 1 - blockIdx.x / a.hkv, it)) return;
+  if (!find_item(a.cu_q, a.nseq, a.tq, fill_tail || a.splits > 1, a.tiles - 1 - blockIdx.x / a.hkv,
+                 [&](int b, int len) { return tiles_of(len) * cuts_of(len, seq_at(a.cu_k, a.nseq, a.tk, b).y); }, it))
+    return;
   const int q0 = it.start, lq = it.len;
   int k0, lk;
   seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
-  const int off = lk - lq, rows = lq * a.group, row0 = it.tile * BM;
-  const int first = row0 + 32 * wave, r = first + (lane & 31);
+  const int cuts = cuts_of(lq, lk), ntile = tiles_of(lq), cut = it.sub / ntile;
+  const int off = lk - lq, rows = lq * a.group, row0 = (it.sub - cut * ntile) * ROWS;
+  const int first = row0 + 32 * wr, r = first + (lane & 31);
   const bool ok = r < rows;
   const int rc = min(r, rows - 1), pos = rc / a.group, g = rc - pos * a.group;
-  // keys a row sees: [0, lim); of the wave's first and last rows, and of the block's last
+  const int heads = a.hkv * a.group;
+  // this block's keys [kbeg, kend) of those that a row sees: [0, limit)
+  const int step = cuts > 1 ? ((lk + cuts - 1) / cuts + BN - 1) / BN * BN : 0, kbeg = cut * step;
   auto limit = [&](int row) {
-    return a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
+    const int n = a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
+    return cuts > 1 ? min(n, kbeg + step) : n;
   };
   const int lim = limit(r), wmin = limit(first), wmax = first < rows ? limit(first + 31) : 0;
-  const int nt = (limit(row0 + BM - 1) + BN - 1) / BN;
+  const int nt = max(0, (limit(row0 + ROWS - 1) - kbeg + BN - 1) / BN);
   Bias bias{};
   if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB, kvh);
 
@@ -84,7 +98,7 @@ __global__ __launch_bounds__(NT, 2) void packed_fwd_kernel(const Args a, int fil
 
   auto fetch = [&](int j) {
     char* buf = smem + (j & 1) * 2 * TB;
-    const int key0 = j * BN, left = lk - key0;
+    const int key0 = kbeg + j * BN, left = lk - key0;
     const i32x4 rk = make_rsrc((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head);
     const i32x4 rv = make_rsrc((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head);
     const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
@@ -104,11 +118,11 @@ __global__ __launch_bounds__(NT, 2) void packed_fwd_kernel(const Args a, int fil
     tile_barrier();
     if (j + 1 < nt) fetch(j + 1);
     const char* buf = smem + (j & 1) * 2 * TB;
-    const int key0 = j * BN;
+    const int key0 = kbeg + j * BN + 32 * NS * wk;
     if (key0 >= wmax) continue;
     f32x16 s[NS];
 #pragma unroll
-    for (int u = 0; u < NS; ++u) s[u] = rows_mma<T, DP>(buf, u, lane, qf);
+    for (int u = 0; u < NS; ++u) s[u] = rows_mma<T, DP>(buf, NS * wk + u, lane, qf);
     if constexpr (BIAS) {
 #pragma unroll
       for (int u = 0; u < NS; ++u) {
@@ -126,7 +140,7 @@ __global__ __launch_bounds__(NT, 2) void packed_fwd_kernel(const Args a, int fil
         }
       }
     }
-    if (key0 + BN > wmin) {
+    if (key0 + 32 * NS > wmin) {
 #pragma unroll
       for (int u = 0; u < NS; ++u)
 #pragma unroll
@@ -160,77 +174,268 @@ __global__ __launch_bounds__(NT, 2) void packed_fwd_kernel(const Args a, int fil
         s[u][i] = __builtin_amdgcn_exp2f(BIAS ? (s[u][i] - mref) * c : fmaf(s[u][i], c, -mc));
         l += s[u][i];
       }
-      cols_mma<T, DP>(buf + TB, u, lane, s[u], o);
+      cols_mma<T, DP>(buf + TB, NS * wk + u, lane, s[u], o);
     }
   }
-
   l = half_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  bool bad = l != l;
+
+  // the log of the softmax's denominator in the backward's units: log2 without, natural with a bias
+  auto lse_of = [&](float mm, float ll, float none) {
+    return ll == 0.f ? none : (BIAS ? mm + __logf(ll) : mm * c + __log2f(ll));
+  };
+  auto head_row = [&](int p, int hd) { return (int64_t)(q0 + p) * heads + kvh * a.group + hd; };
+  // four results of a row: the output, or this cut's part of it
+  auto put = [&](int64_t at, int p, int hd, int d, f32x4 x) {
+    if (cuts > 1) {
+      *reinterpret_cast<f32x4*>(a.part + ((int64_t)cut * a.tq * heads + at) * a.dim + d) = x;
+    } else {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 w;
 #pragma unroll
-  for (int t = 0; t < TL::ND; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      o[t][i] *= inv;
-      bad |= o[t][i] != o[t][i];
+      for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(x[i]);
+      *reinterpret_cast<T4*>((T*)a.out + (int64_t)(q0 + p) * a.o_row + (kvh * a.group + hd) * a.o_head + d) = w;
     }
-  if (ok) {
-    T* op = (T*)a.out + (int64_t)(q0 + pos) * a.o_row + (kvh * a.group + g) * a.o_head;
+  };
+  auto put_lse = [&](int64_t at, float mm, float ll) {
+    if (cuts > 1) a.part_lse[(int64_t)cut * a.tq * heads + at] = lse_of(mm, ll, -INFINITY);
+    else if (a.lse) a.lse[at] = lse_of(mm, ll, INFINITY);
+    if (a.splits > 1 && cut == 0) a.part_n[at] = cuts;
+  };
+  const bool write = it.b < a.nseq || fill_tail;
+
+  if constexpr (WK == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bool bad = l != l;
+    const int64_t at = head_row(pos, g);
 #pragma unroll
     for (int t = 0; t < TL::ND; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 32 * t + 8 * e + 4 * h;
-        if (d < a.dim) {
-          typedef T T4 __attribute__((ext_vector_type(4)));
-          T4 w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(o[t][4 * e + i]);
-          *reinterpret_cast<T4*>(op + d) = w;
-        }
+      for (int i = 0; i < 16; ++i) {
+        o[t][i] *= inv;
+        bad |= o[t][i] != o[t][i];
       }
-    // for the backward, in the units of its exponent: log2 without, natural with a bias
-    if (a.lse && h == 0)
-      a.lse[(int64_t)(q0 + pos) * a.hkv * a.group + kvh * a.group + g] =
-          l == 0.f ? INFINITY : (BIAS ? m + __logf(l) : m * c + __log2f(l));
-  }
-  unsigned long long redo = __ballot(bad && ok);
-  redo |= redo >> 32;
-  for (unsigned left = (unsigned)redo; left; left &= left - 1) {
-    const int row = first + __builtin_ctz(left), rp = row / a.group;
-    slow_row<T, BIAS>(a, bias, kvh, row - rp * a.group, rp, q0, k0, lk, limit(row), off);
+    if (ok) {
+      if (write)
+#pragma unroll
+        for (int t = 0; t < TL::ND; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = 32 * t + 8 * e + 4 * h;
+            if (d < a.dim) put(at, pos, g, d, f32x4{o[t][4 * e], o[t][4 * e + 1], o[t][4 * e + 2], o[t][4 * e + 3]});
+          }
+      if (h == 0) put_lse(at, m, l);
+    }
+    if (cuts > 1) return;   // packed_join_kernel looks for NaN
+    unsigned long long redo = __ballot(bad && ok);
+    redo |= redo >> 32;
+    for (unsigned left = (unsigned)redo; left; left &= left - 1) {
+      const int row = first + __builtin_ctz(left), rp = row / a.group;
+      const int hd = row - rp * a.group;
+      slow_row<T>(a, kvh, hd, rp, q0, k0, limit(row), [&](int j) {
+        return BIAS ? bias.tab[hd * bias.nb + bias.bucket(j - rp - off)] : 0.f;
+      });
+    }
+  } else {
+    // join the WK waves of each 32 rows through LDS
+    __syncthreads();
+    float* oo = reinterpret_cast<float*>(smem);
+    float *mm = oo + 4 * 32 * OP, *ll = mm + 128;
+    int* redo = reinterpret_cast<int*>(ll + 128);
+    const int x = wave * 32 + (lane & 31);
+#pragma unroll
+    for (int t = 0; t < TL::ND; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(oo + x * OP + 32 * t + 8 * e + 4 * h) =
+            f32x4{o[t][4 * e], o[t][4 * e + 1], o[t][4 * e + 2], o[t][4 * e + 3]};
+    if (h == 0) {
+      mm[x] = m;
+      ll[x] = l;
+    }
+    if (threadIdx.x < ROWS) redo[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < ROWS * (DP / 4); i += NT) {
+      const int jr = i / (DP / 4), d = (i - jr * (DP / 4)) * 4, row = row0 + jr;
+      if (row >= rows || d >= a.dim) continue;
+      const int w0 = (jr >> 5) * WK * 32 + (jr & 31), rp = row / a.group, hd = row - rp * a.group;
+      float top = mm[w0];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) top = fmaxf(top, mm[w0 + 32 * w]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      float tot = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float f = __builtin_amdgcn_exp2f((mm[w0 + 32 * w] - ref) * c);
+        tot = fmaf(ll[w0 + 32 * w], f, tot);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(oo + (w0 + 32 * w) * OP + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[e], f, sum[e]);
+      }
+      const float inv = tot == 0.f ? 0.f : 1.f / tot;
+      bool bad = tot != tot;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sum[e] *= inv;
+        bad |= sum[e] != sum[e];
+      }
+      const int64_t at = head_row(rp, hd);
+      if (write) put(at, rp, hd, d, sum);
+      if (d == 0) put_lse(at, top, tot);
+      if (bad) redo[jr] = 1;
+    }
+    if (cuts > 1) return;
+    __syncthreads();
+    for (int jr = wave; jr < min(ROWS, rows - row0); jr += 4) {
+      if (!redo[jr]) continue;
+      const int row = row0 + jr, rp = row / a.group;
+      const int hd = row - rp * a.group;
+      slow_row<T>(a, kvh, hd, rp, q0, k0, limit(row), [&](int j) {
+        return BIAS ? bias.tab[hd * bias.nb + bias.bucket(j - rp - off)] : 0.f;
+      });
+    }
   }
 }
 
+// rows whose keys were cut: out = sum of the parts weighted by exp(lse - the largest), four elements
+// a thread, in the order of the cuts
 template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
+  constexpr int TPR = DP / 4;   // threads of a row
+  const int heads = a.hkv * a.group;
+  const int64_t all = (int64_t)a.tq * heads;
+  const int64_t at = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const int d = (threadIdx.x % TPR) * 4;
+  const int n = at < all ? min(a.part_n[at], a.splits) : 1;
+  bool bad = false;
+  if (n > 1) {
+    float top = -INFINITY;
+    for (int i = 0; i < n; ++i) top = fmaxf(top, a.part_lse[i * all + at]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float tot = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float x = (a.part_lse[i * all + at] - ref) * (BIAS ? LOG2E : 1.f);
+      const float f = __builtin_amdgcn_exp2f(x);
+      tot += f;
+      if (d < a.dim) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + (i * all + at) * a.dim + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[e], f, sum[e]);
+      }
+    }
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
+    bad = tot != tot;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum[e] *= inv;
+      bad |= sum[e] != sum[e];
+    }
+    if (d < a.dim) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      T4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(sum[e]);
+      const int64_t row = at / heads;
+      *reinterpret_cast<T4*>((T*)a.out + row * a.o_row + (at - row * heads) * a.o_head + d) = w;
+    }
+    if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : (BIAS ? ref + __logf(tot) : ref + __log2f(tot));
+  }
+  if (!__ballot(bad)) return;
+  // NaN: the wave's rows one by one (each wave for itself: no barrier past this point but its own)
+  const int lane = threadIdx.x & 63;
+  for (int rr = 0; rr < 64 / TPR; ++rr) {
+    const bool mine = lane / TPR == rr;
+    if (!__ballot(bad && mine)) continue;
+    const int64_t row_at = (int64_t)blockIdx.x * (NT / TPR) + (threadIdx.x >> 6) * (64 / TPR) + rr;
+    const int row = (int)(row_at / heads), head = (int)(row_at - (int64_t)row * heads);
+    int b = 0;
+    while (b < a.nseq && clampi(a.cu_q[b + 1], 0, a.tq) <= row) ++b;
+    if (b == a.nseq) continue;
+    const int2 qs = seq_at(a.cu_q, a.nseq, a.tq, b), ks = seq_at(a.cu_k, a.nseq, a.tk, b);
+    const int pos = row - qs.x, off = ks.y - qs.y;
+    slow_row<T>(a, head / a.group, head % a.group, pos, qs.x, ks.x, a.causal ? clampi(pos + off + 1, 0, ks.y) : ks.y,
+                [&](int j) {
+                  if (!BIAS) return 0.f;
+                  const int rel = j - pos - off, n = a.both ? abs(rel) : max(-rel, 0);
+                  int bk = a.both && rel > 0 ? a.buckets / 2 : 0;
+                  for (int e = 0; e < a.nedge; ++e) bk += a.edge[e] <= n;
+                  const int64_t x = (int64_t)bk * heads + head;
+                  return a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[x]
+                                    : to_f32(reinterpret_cast<const T*>(a.bias)[x]);
+                });
+  }
+}
+
+// Which shape a call runs in. Lengths are on the device, so the rule goes by totals.
+struct Plan { int wk, chunk, splits, items; };
+static Plan plan_of(const dp_packed_attn* d) {
+  const int64_t group = d->heads / d->kv_heads, rows = d->tq * group, seqs = std::max(1, d->nseq);
+  Plan p{1, 0, 1, 0};
+  const int64_t wide = (rows / BM + 1) * d->kv_heads;   // blocks at least
+  const bool few = rows <= 32 * seqs;
+  if (few || (wide < 256 && d->tk <= 2048 * seqs)) p.wk = d->dtype == DP_F32 && d->dim > 64 ? 2 : 4;
+  const int per = BM / p.wk;
+  int64_t items = rows / per + d->nseq + 1;
+  if (d->tk > 1024 && (few || (rows / per + 1) * d->kv_heads < 256) && d->tq > 0) {
+    // about 1024 blocks of few rows, or 512 of many; a part of the output is written in f32 per cut and row, so a
+    // cut has at least 16 keys a row (splits_of)
+    const int64_t target = few ? 1024 : 512;
+    const int64_t most_tiles = rows / per + 1;             // of one sequence
+    int64_t chunk = std::max<int64_t>(256, (int64_t)d->tk * d->kv_heads * (few ? 1 : (items + seqs) / seqs) / target);
+    chunk = (chunk + 127) / 128 * 128;
+    int64_t splits = std::min<int64_t>(64, (d->tk + chunk - 1) / chunk);
+    splits = std::min(splits, std::max<int64_t>(1, (few ? 64 : 4) * target / std::max<int64_t>(1, rows / per * d->kv_heads)));
+    splits = std::min(splits, std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)d->tq * d->heads * (d->dim + 1) * 4)));
+    if (splits > 1) {
+      p.chunk = (int)chunk;
+      p.splits = (int)splits;
+      // sum of tiles x cuts: cuts <= splits, and <= 1 + keys / chunk
+      items = std::min(items * splits, items + most_tiles * (d->tk / chunk + 1));
+    }
+  }
+  p.items = (int)std::min<int64_t>(items, INT32_MAX);
+  return p;
+}
+
+template <typename T, int DP, int WK, bool BIAS>
 int launch(const Args& a, int fill_tail, hipStream_t s) {
-  constexpr int BN = sizeof(T) == 2 ? 64 : 32;
+  constexpr int BN = WK > 1 ? 32 * WK : sizeof(T) == 2 ? 64 : 32;
   const int lds = 4 * BN * Tile<T, DP>::RB + bias_lds(a);
-  const auto kern = packed_fwd_kernel<T, DP, BN, BIAS>;
+  const auto kern = packed_fwd_kernel<T, DP, WK, BN, BIAS>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     DP_REQUIRE(e == hipSuccess, "dp_packed_attn_fwd: %d bytes of LDS: %s", lds, hipGetErrorString(e));
   }
   hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a, fill_tail);
+  if (a.splits > 1) {
+    const int64_t n = (int64_t)a.tq * a.hkv * a.group, per = NT / (DP / 4);
+    hipLaunchKernelGGL((packed_join_kernel<T, DP, BIAS>), dim3((unsigned)((n + per - 1) / per)), dim3(NT), 0, s, a);
+  }
   return dp_check_launch("dp_packed_attn_fwd");
 }
 
 template <typename T, bool BIAS>
-int launch_dim(const Args& a, int fill_tail, hipStream_t s) {
-  if (a.dim <= 32) return launch<T, 32, BIAS>(a, fill_tail, s);
-  if (a.dim <= 64) return launch<T, 64, BIAS>(a, fill_tail, s);
-  return launch<T, 128, BIAS>(a, fill_tail, s);
+int launch_dim(const Args& a, int wk, int fill_tail, hipStream_t s) {
+  constexpr int W128 = sizeof(T) == 2 ? 4 : 2;
+  if (a.dim <= 32) return wk > 1 ? launch<T, 32, 4, BIAS>(a, fill_tail, s) : launch<T, 32, 1, BIAS>(a, fill_tail, s);
+  if (a.dim <= 64) return wk > 1 ? launch<T, 64, 4, BIAS>(a, fill_tail, s) : launch<T, 64, 1, BIAS>(a, fill_tail, s);
+  return wk > 1 ? launch<T, 128, W128, BIAS>(a, fill_tail, s) : launch<T, 128, 1, BIAS>(a, fill_tail, s);
 }
 
 }  // namespace
 
-int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what, bool backward);
+
+int64_t dp_packed_bwd_ws_bytes(const dp_packed_attn* d);   // packed_attn_bwd.hip
 
 extern "C" int64_t dp_packed_attn_ws_bytes(const dp_packed_attn* d, int32_t backward) {
-  if (!d || d->heads <= 0 || d->kv_heads <= 0 || d->tq < 0) return 0;
-  if (!backward) return 0;
-  const int64_t tiles = (int64_t)d->tq * (d->heads / d->kv_heads) / BM + d->nseq + 1;
-  return ((int64_t)d->tq * d->heads + (d->bias ? tiles * d->heads * d->buckets : 0)) * 4;
+  if (!d || d->heads <= 0 || d->kv_heads <= 0 || d->tq < 0 || d->tk < 0 || d->nseq < 0) return 0;
+  if (!backward) {
+    const Plan p = plan_of(d);
+    return p.splits > 1 ? (int64_t)d->tq * d->heads * (p.splits * ((int64_t)d->dim + 1) + 1) * 4 : 0;
+  }
+  return dp_packed_bwd_ws_bytes(d);
 }
 
 // the checks that forward and backward share, and the kernels' form of the descriptor
@@ -287,8 +492,23 @@ extern "C" int dp_packed_attn_fwd(const dp_packed_attn* d, void* stream) {
   Args a;
   if (const int rc = dp_packed_attn_args(d, &a, "dp_packed_attn_fwd", false)) return rc;
   if (a.tq == 0) return 0;
+  const int64_t need = dp_packed_attn_ws_bytes(d, 0);
+  DP_REQUIRE(d->ws_bytes >= need && (d->ws || !need), "dp_packed_attn_fwd: workspace holds %lld bytes, needs %lld",
+             (long long)d->ws_bytes, (long long)need);
+  const Plan p = plan_of(d);
+  DP_REQUIRE((int64_t)p.items * a.hkv < INT32_MAX, "dp_packed_attn_fwd: too many tiles");
+  a.tiles = p.items;
+  a.chunk = p.chunk;
+  a.splits = p.splits;
+  if (p.splits > 1) {
+    const int64_t n = (int64_t)a.tq * d->heads;
+    a.part = (float*)d->ws;
+    a.part_lse = a.part + n * p.splits * d->dim;
+    a.part_n = (int*)(a.part_lse + n * p.splits);
+  }
   hipStream_t s = as_stream(stream);
+  const int f = d->fill_tail;
   if (d->dtype == DP_BF16)
-    return a.bias ? launch_dim<bf16_t, true>(a, d->fill_tail, s) : launch_dim<bf16_t, false>(a, d->fill_tail, s);
-  return a.bias ? launch_dim<float, true>(a, d->fill_tail, s) : launch_dim<float, false>(a, d->fill_tail, s);
+    return a.bias ? launch_dim<bf16_t, true>(a, p.wk, f, s) : launch_dim<bf16_t, false>(a, p.wk, f, s);
+  return a.bias ? launch_dim<float, true>(a, p.wk, f, s) : launch_dim<float, false>(a, p.wk, f, s);
 }

@@ -250,6 +250,53 @@ def test_forward_backward(shape, dtype):
         _check(got[n], want[n], n)
 
 
+# keys cut into parts that are joined: single tokens and chunks over long caches, few long sequences
+LONG = [
+    (8, 2, 128, [1, 1, 0, 1, 3], [5000, 1, 40, 2311, 700], True, 0),
+    (4, 4, 64, [1, 2], [3001, 1500], True, 16),
+    (2, 1, 32, [1], [9000], False, 0),
+    (8, 2, 128, [200, 3], [4100, 1700], True, 0),
+    (4, 2, 64, [300], [2500], False, 32),
+    (2, 2, 96, [1300], [1300], True, 0),
+    (6, 2, 64, [3, 2100], [10, 2100], True, 8),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: f"h{s[0]}k{s[1]}d{s[2]}b{s[6]}q{max(s[3])}k{max(s[4])}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_long_keys(shape, dtype):
+    heads, hk, d, ql, kl, causal, nb = shape
+    q, k, v, dout, t = _inputs(d + nb, dtype, heads, hk, d, ql, kl, nb, extra=5)
+    got = _run(q, k, v, dout, ql, kl, t, causal=causal)
+    want = _reference(q, k, v, ql, kl, causal, d ** -0.5, t, 128, not causal, dout)
+    for n in want:
+        _check(got[n], want[n], n)
+    n, m = sum(ql), sum(kl)
+    out = torch.full_like(q, 3.0)
+    with torch.no_grad():
+        A.packed_attention(q, k, v, _cu(ql), _cu(kl), causal=causal, bias_table=t, out=out)
+    assert torch.equal(out[:n], got["out"][:n]) and (out[n:] == 3).all()
+    assert not got["out"][n:].any() and not got["dk"][m:].any() and not got["dv"][m:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("nb", [0, 8])
+def test_hidden_values_with_long_keys(dtype, nb):
+    """The last key, seen by the last query alone, is inf: the other queries do not change (their rows
+    are computed again key by key, which moves them by roundings only)."""
+    for ql, kl in (([3], [3000]), ([150], [3000])):
+        q, k, v, _, t = _inputs(12, dtype, 4, 2, 64, ql, kl, nb)
+        kw = dict(causal=True, bias_table=t)
+        base = A.packed_attention(q, k, v, _cu(ql), _cu(kl), **kw)
+        v[-1] = float("inf")
+        got = A.packed_attention(q, k, v, _cu(ql), _cu(kl), **kw)
+        lim = 4 * HALF[dtype] * base.double().abs() + 2e-5 * (dtype == torch.float32) + 2e-2 * (dtype != torch.float32)
+        assert ((got.double() - base.double()).abs() <= lim)[:-1].all()
+        assert got[-1].isinf().all()
+
+
 BIASED = [
     (4, 4, 32, [18, 300, 1, 77], None, False, 32, 128, None),
     (4, 2, 64, [200, 65, 129], None, True, 32, 128, None),
