@@ -121,6 +121,25 @@ __device__ __forceinline__ f32x16 rows_mma(const char* tile, int sub, int lane, 
   return c;
 }
 
+// the same for N subtiles from sub on, their chains of products side by side
+template <typename T, int DP, int N>
+__device__ __forceinline__ void rows_mma_n(const char* tile, int sub, int lane, const u32x4 (&b)[Tile<T, DP>::KS],
+                                           f32x16 (&c)[N]) {
+  using TL = Tile<T, DP>;
+  const int row = lane & 31, h = lane >> 5;
+  const char* base = tile + (32 * sub + row) * TL::RB;
+  const int f = TL::swz(row);
+#pragma unroll
+  for (int u = 0; u < N; ++u) c[u] = zero16();
+#pragma unroll
+  for (int s = 0; s < TL::KS; ++s)
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const u32x4 a = *reinterpret_cast<const u32x4*>(base + 32 * u * TL::RB + (((2 * s + h) ^ f) << 4));
+      c[u] = mma_step<T>(a, b[s], c[u]);
+    }
+}
+
 // acc[t] += tile^T (columns 32 t ...) x p, contracted over the tile's rows 32 sub .. 32 sub + 31
 template <typename T, int DP>
 __device__ __forceinline__ void cols_mma(const char* tile, int sub, int lane, const f32x16& p,
@@ -178,6 +197,32 @@ __device__ __forceinline__ void stage(const i32x4& rsrc, char* tile, int dim, OF
     dma16(rsrc, tile + (it * NT + wave * 64) * 16, o >= 0 && c * TL::VN < dim ? o + c * 16 : OOB);
   }
 }
+
+// ROWS rows, stride bytes apart, of which the first `valid` exist: one lane offset serves every pass (the
+// rows of two passes are a multiple of 8 apart, so a chunk's place is the same), the passes advance
+// the descriptor's base, and its length ends with the last row. lane_off(): that offset.
+template <typename T, int DP>
+__device__ __forceinline__ int lane_off(int stride, int dim) {
+  using TL = Tile<T, DP>;
+  static_assert(NT / TL::CPR % 8 == 0, "whole swizzle periods a pass");
+  const int row = threadIdx.x / TL::CPR, c = (threadIdx.x % TL::CPR) ^ TL::swz(row);
+  return c * TL::VN < dim ? row * stride + c * 16 : OOB;
+}
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void stage_rows(const T* base, int stride, int valid, char* tile, int dim, int off,
+                                           int wave) {
+  using TL = Tile<T, DP>;
+  constexpr int RPP = NT / TL::CPR;   // rows of a pass
+  const int end = (min(valid, ROWS) - 1) * stride + dim * (int)sizeof(T);   // below 2^31: stride < 2^24
+#pragma unroll
+  for (int it = 0; it < ROWS / RPP; ++it) {
+    i32x4 r = make_rsrc(reinterpret_cast<const char*>(base) + (int64_t)it * RPP * stride);
+    r[2] = max(end - it * RPP * stride, 0);
+    dma16(r, tile + (it * NT + wave * 64) * 16, off);
+  }
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // the lane's fragments of one global row as a B operand (zero when !ok and past dim)
 template <typename T, int DP>

@@ -28,9 +28,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
   static_assert(WK == 1 || 4 * TB >= 4 * 32 * OP * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform: scalar branches below
   const int wk = wave % WK, wr = wave / WK;
-  const int kvh = blockIdx.x % a.hkv, tile = a.tiles - 1 - blockIdx.x / a.hkv;
+  const int kvh = uniform(blockIdx.x % a.hkv), tile = a.tiles - 1 - blockIdx.x / a.hkv;
   const int heads = a.hkv * a.group;
   float* part = BIAS ? a.dbias_part + ((int64_t)tile * a.hkv + kvh) * a.group * a.buckets : nullptr;
   Item it;
@@ -49,8 +50,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   auto limit = [&](int row) {
     return a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
   };
-  const int lim = limit(r), wmin = limit(first), wmax = first < rows ? limit(first + 31) : 0;
-  const int nt = (limit(row0 + ROWS - 1) + BN - 1) / BN;
+  const int lim = limit(r), wmin = uniform(limit(first)), wmax = uniform(first < rows ? limit(first + 31) : 0);
+  const int nt = uniform((limit(row0 + ROWS - 1) + BN - 1) / BN);
+  // positions of the wave's first and last row
+  const int pfirst = uniform(first / a.group + off), plast = uniform(min(first + 31, rows - 1) / a.group + off);
   Bias bias{};
   float* bins = nullptr;
   if constexpr (BIAS) {
@@ -80,14 +83,15 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   if (ok && h == 0 && wk == 0) a.dsum[at] = D;
   const float lse = ok ? a.lse[at] : INFINITY;
 
+  const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
+  const int koff = lane_off<T, DP>(ks, a.dim), voff = lane_off<T, DP>(vs, a.dim);
   auto fetch = [&](int j) {
     char* buf = smem + (j & 1) * 2 * TB;
     const int key0 = j * BN, left = lk - key0;
-    const i32x4 rk = make_rsrc((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head);
-    const i32x4 rv = make_rsrc((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head);
-    const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
-    stage<T, DP, BN>(rk, buf, a.dim, [&](int row) { return row < left ? row * ks : -1; });
-    stage<T, DP, BN>(rv, buf + TB, a.dim, [&](int row) { return row < left ? row * vs : -1; });
+    stage_rows<T, DP, BN>((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head, ks, left, buf, a.dim, koff,
+                          wave);
+    stage_rows<T, DP, BN>((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head, vs, left, buf + TB, a.dim,
+                          voff, wave);
   };
 
   const float c = a.scale * LOG2E;
@@ -111,8 +115,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
       const f32x16 dp = rows_mma<T, DP>(buf + TB, u, lane, gf);
       int one = -1;
       if constexpr (BIAS) {
-        const int pl = min(first + 31, rows - 1) / a.group + off, pf = first / a.group + off;
-        one = bias.one_bucket(k32 - pl, k32 + 31 - pf);
+        one = bias.one_bucket(k32 - plast, k32 + 31 - pfirst);
         const float* tab = bias.tab + g * bias.nb;
         if (one >= 0) {
           const float b = tab[one];
@@ -246,8 +249,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   float* dsum_s = lse_s + 2 * BR;
   int* pos_s = reinterpret_cast<int*>(dsum_s + 2 * BR);
   int* head_s = pos_s + 2 * BR;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int kvh = blockIdx.x % a.hkv;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform: scalar branches below
+  const int kvh = uniform(blockIdx.x % a.hkv);
   const int heads = a.hkv * a.group;
   auto tiles_of = [&](int len) { return (len + BM - 1) / BM; };
   Item it;
@@ -260,15 +264,15 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   int q0, lq;
   seq_of(a.cu_q, a.nseq, a.tq, it.b, q0, lq);
   const int off = lk - lq, rows = lq * a.group, ntile = tiles_of(lk);
-  const int cuts = cuts_of(a, rows), cut = it.sub / ntile, tile = it.sub - cut * ntile;
+  const int cuts = uniform(cuts_of(a, rows)), cut = uniform(it.sub / ntile), tile = it.sub - cut * ntile;
   const int first = tile * BM + 32 * wave, key = first + (lane & 31);
   const bool ok = key < lk;
   // the first row that sees a key
   auto sees = [&](int kk) { return a.causal ? max(0, kk - off) * a.group : 0; };
-  const int mine = sees(key), wfirst = sees(first), wlast = sees(min(first + 31, lk - 1));
+  const int mine = sees(key), wfirst = uniform(sees(first)), wlast = uniform(sees(min(first + 31, lk - 1)));
   // this block's rows [start, end)
   const int seen = sees(tile * BM) / 32 * 32, step = cuts > 1 ? cut_step(rows, cuts) : 0;
-  const int start = max(seen, cut * step), end = cuts > 1 ? min(rows, (cut + 1) * step) : rows;
+  const int start = uniform(max(seen, cut * step)), end = uniform(cuts > 1 ? min(rows, (cut + 1) * step) : rows);
   if (start >= end && cuts > 1) return;
   Bias bias{};
   if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB + 16 * BR * 2, kvh);

@@ -63,9 +63,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
   static_assert(WK == 1 || 4 * TB >= (4 * 32 * (OP + 2) + 2 * ROWS) * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform: scalar branches below
   const int wk = wave % WK, wr = wave / WK;
-  const int kvh = blockIdx.x % a.hkv;
+  const int kvh = uniform(blockIdx.x % a.hkv);
   auto tiles_of = [&](int len) { return (len * a.group + ROWS - 1) / ROWS; };
   auto cuts_of = [&](int lq, int lk) { return splits_of(a, lk, min(ROWS, lq * a.group)); };
   Item it;
@@ -76,34 +77,37 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   const int q0 = it.start, lq = it.len;
   int k0, lk;
   seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
-  const int cuts = cuts_of(lq, lk), ntile = tiles_of(lq), cut = it.sub / ntile;
+  const int cuts = uniform(cuts_of(lq, lk)), ntile = uniform(tiles_of(lq)), cut = uniform(it.sub / ntile);
   const int off = lk - lq, rows = lq * a.group, row0 = (it.sub - cut * ntile) * ROWS;
   const int first = row0 + 32 * wr, r = first + (lane & 31);
   const bool ok = r < rows;
   const int rc = min(r, rows - 1), pos = rc / a.group, g = rc - pos * a.group;
   const int heads = a.hkv * a.group;
   // this block's keys [kbeg, kend) of those that a row sees: [0, limit)
-  const int step = cuts > 1 ? ((lk + cuts - 1) / cuts + BN - 1) / BN * BN : 0, kbeg = cut * step;
+  const int step = uniform(cuts > 1 ? ((lk + cuts - 1) / cuts + BN - 1) / BN * BN : 0), kbeg = cut * step;
   auto limit = [&](int row) {
     const int n = a.causal ? clampi(min(row, rows - 1) / a.group + off + 1, 0, lk) : lk;
     return cuts > 1 ? min(n, kbeg + step) : n;
   };
-  const int lim = limit(r), wmin = limit(first), wmax = first < rows ? limit(first + 31) : 0;
-  const int nt = max(0, (limit(row0 + ROWS - 1) - kbeg + BN - 1) / BN);
+  const int lim = limit(r), wmin = uniform(limit(first)), wmax = uniform(first < rows ? limit(first + 31) : 0);
+  const int nt = uniform(max(0, (limit(row0 + ROWS - 1) - kbeg + BN - 1) / BN));
+  // positions of the wave's first and last row
+  const int pfirst = uniform(first / a.group + off), plast = uniform(min(first + 31, rows - 1) / a.group + off);
   Bias bias{};
   if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB, kvh);
 
   u32x4 qf[TL::KS];
   load_frags<T, DP>((const T*)a.q + (int64_t)(q0 + pos) * a.q_row + (kvh * a.group + g) * a.q_head, ok, a.dim, h, qf);
 
+  const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
+  const int koff = lane_off<T, DP>(ks, a.dim), voff = lane_off<T, DP>(vs, a.dim);
   auto fetch = [&](int j) {
     char* buf = smem + (j & 1) * 2 * TB;
     const int key0 = kbeg + j * BN, left = lk - key0;
-    const i32x4 rk = make_rsrc((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head);
-    const i32x4 rv = make_rsrc((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head);
-    const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
-    stage<T, DP, BN>(rk, buf, a.dim, [&](int row) { return row < left ? row * ks : -1; });
-    stage<T, DP, BN>(rv, buf + TB, a.dim, [&](int row) { return row < left ? row * vs : -1; });
+    stage_rows<T, DP, BN>((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head, ks, left, buf, a.dim, koff,
+                          wave);
+    stage_rows<T, DP, BN>((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head, vs, left, buf + TB, a.dim,
+                          voff, wave);
   };
 
   // scores in units in which exp(s - m) = exp2((s - m) c): raw products, or, with a bias, scaled ones
@@ -121,13 +125,11 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
     const int key0 = kbeg + j * BN + 32 * NS * wk;
     if (key0 >= wmax) continue;
     f32x16 s[NS];
-#pragma unroll
-    for (int u = 0; u < NS; ++u) s[u] = rows_mma<T, DP>(buf, NS * wk + u, lane, qf);
+    rows_mma_n<T, DP, NS>(buf, NS * wk, lane, qf, s);
     if constexpr (BIAS) {
 #pragma unroll
       for (int u = 0; u < NS; ++u) {
-        const int k32 = key0 + 32 * u, pl = min(first + 31, rows - 1) / a.group + off, pf = first / a.group + off;
-        const int one = bias.one_bucket(k32 - pl, k32 + 31 - pf);
+        const int k32 = key0 + 32 * u, one = bias.one_bucket(k32 - plast, k32 + 31 - pfirst);
         const float* tab = bias.tab + g * bias.nb;
         if (one >= 0) {
           const float b = tab[one];
