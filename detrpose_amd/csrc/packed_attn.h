@@ -16,8 +16,8 @@
 // Tiles. Rows of DP elements (dim padded to 32, 64 or 128; the padding reads as zero), filled by
 // direct HBM -> LDS loads whose buffer descriptor returns zero for rows outside the sequence: what
 // lies there (another sequence, an unwritten cache row) never enters a product. A row's 16-byte chunks
-// are permuted by its number (swz) so that both read patterns spread over all banks; the permutation
-// is applied to the global address, because the LDS side of such a load is contiguous per wave.
+// are permuted by its number (Tile::swz); the permutation is applied to the global address, because
+// the LDS side of such a load is contiguous per wave.
 #pragma once
 #include "common.h"
 #include "conv_lds.h"
@@ -77,11 +77,20 @@ struct Tile {
   static constexpr int RB = DP * (int)sizeof(T);
   static constexpr int KS = CPR / 2;            // chunk pairs: the steps of a product over dim
   static constexpr int ND = DP / 32;            // 32-wide column tiles
-  // the chunk permutation of a row: consecutive rows' equal chunks, and the chunk pairs of 4
-  // consecutive rows, land on different 16-byte slots of the 128-byte bank line
+  // A tile lies in groups of 1 KB (what one wave's load writes) GS bytes apart, and a row's chunks are
+  // permuted by swz, so that over the 16 slots of 16 bytes that one LDS cycle serves, the equal chunks of 16
+  // rows (products over dim) and what one column read takes at once (bf16: 64 bytes of each of 4
+  // rows; f32: 128 bytes of rows r and r + 4) lie on different slots. The groups' spacing takes part of
+  // that from the permutation, which leaves few different addresses to keep in registers.
+  static constexpr int RG = 1024 / RB, GS = 1040;
+  static constexpr int PERIOD = sizeof(T) == 2 || CPR == 8 ? RG : 8;   // of swz, in rows
   __device__ static __forceinline__ int swz(int row) {
-    return CPR >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : (((row & 2)) | ((row >> 2) & 1));
+    if (sizeof(T) == 2) return CPR == 16 ? (row & 3) << 2 : CPR == 8 ? ((row & 2) << 1) | ((row & 4) >> 1) : (row >> 2) & 3;
+    if (CPR == 32) return ((row ^ (row >> 2)) & 1) << 3;
+    return CPR == 16 ? ((row & 3) << 2) ^ ((row & 4) << 1) : ((row & 2) << 1) | ((row & 4) >> 1);
   }
+  __device__ static __forceinline__ int off(int row) { return row / RG * GS + row % RG * RB; }
+  static constexpr int bytes(int rows) { return rows / RG * GS; }
 };
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -105,74 +114,105 @@ __device__ __forceinline__ f32x16 mma_step(const u32x4& a, const u32x4& b, f32x1
   }
 }
 
-// tile rows (32 sub + l & 31) x the lane's column fragments
+// a lane's operands for products over dim: its chunk of step s of row 32 u + (l & 31). swz leaves the low
+// bit (and with 16 chunks a row the low two) of a chunk alone, so the steps share few addresses
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 rows_mma(const char* tile, int sub, int lane, const u32x4 (&b)[Tile<T, DP>::KS]) {
+struct RowReader {
   using TL = Tile<T, DP>;
-  const int row = lane & 31, h = lane >> 5;
-  const char* base = tile + (32 * sub + row) * TL::RB;
-  const int f = TL::swz(row);
-  f32x16 c = zero16();
-#pragma unroll
-  for (int s = 0; s < TL::KS; ++s) {
-    const u32x4 a = *reinterpret_cast<const u32x4*>(base + (((2 * s + h) ^ f) << 4));
-    c = mma_step<T>(a, b[s], c);
+  static constexpr int SH = sizeof(T) == 2 && TL::CPR == 16 ? 2 : sizeof(T) == 2 && TL::CPR == 4 ? 0 : 1;
+  const char* base;
+  int f, h;
+  __device__ __forceinline__ RowReader(const char* tile, int lane)
+      : base(tile + TL::off(lane & 31) + (SH ? (lane >> 5) * 16 : 0)), f(TL::swz(lane & 31)), h(SH ? 0 : lane >> 5) {}
+  __device__ __forceinline__ bf16x8 read(int u, int s) const {
+    const int c = 2 * s + h, lo = c & ((1 << SH) - 1);
+    return *reinterpret_cast<const bf16x8*>(base + TL::bytes(32) * u + lo * 16 + (((c - lo) ^ f) << 4));
   }
-  return c;
-}
+};
 
-// the same for N subtiles from sub on, their chains of products side by side
+// bf16: columns 32 t + (l & 31) of rows 32 u + 16 m + (the step's slots), transposed by the read
+template <int DP>
+struct ColReader {
+  using TL = Tile<bf16_t, DP>;
+  // the second four rows of a step are 8 further on
+  static constexpr int D8 = TL::RG <= 8 ? 8 / TL::RG * TL::GS : 8 * TL::RB, D16 = 16 / TL::RG * TL::GS;
+  static constexpr bool WHOLE = TL::CPR == 16;   // swz permutes whole column tiles
+  const char* base;
+  int f, f8, c;
+  __device__ __forceinline__ ColReader(const char* tile, int lane) {
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), p4 = lane & 3;   // r: row % 8 of every row read
+    c = 2 * ((lane >> 4) & 1) + (p4 >> 1);
+    base = tile + TL::off(r) + (p4 & 1) * 8 + (WHOLE ? c * 16 : 0);
+    f = TL::swz(r);
+    f8 = TL::RG <= 8 ? f : TL::swz(r + 8);
+    if (WHOLE) c = 0;
+  }
+  __device__ __forceinline__ bf16x8 read(int u, int m, int t) const {
+    const char* at = base + TL::bytes(32) * u + m * D16;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(at + (((4 * t + c) ^ f) << 4)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(at + D8 + (((4 * t + c) ^ f8) << 4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  }
+};
+
+// c[u] = rows 32 (sub + u) ... of the tile x the lane's column fragments, the N chains side by side
 template <typename T, int DP, int N>
 __device__ __forceinline__ void rows_mma_n(const char* tile, int sub, int lane, const u32x4 (&b)[Tile<T, DP>::KS],
                                            f32x16 (&c)[N]) {
   using TL = Tile<T, DP>;
-  const int row = lane & 31, h = lane >> 5;
-  const char* base = tile + (32 * sub + row) * TL::RB;
-  const int f = TL::swz(row);
+  const RowReader<T, DP> rd(tile + TL::bytes(32) * sub, lane);
 #pragma unroll
   for (int u = 0; u < N; ++u) c[u] = zero16();
 #pragma unroll
   for (int s = 0; s < TL::KS; ++s)
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(base + 32 * u * TL::RB + (((2 * s + h) ^ f) << 4));
-      c[u] = mma_step<T>(a, b[s], c[u]);
-    }
+    for (int u = 0; u < N; ++u) c[u] = mma_step<T>(__builtin_bit_cast(u32x4, rd.read(u, s)), b[s], c[u]);
+}
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 rows_mma(const char* tile, int sub, int lane, const u32x4 (&b)[Tile<T, DP>::KS]) {
+  f32x16 c[1];
+  rows_mma_n<T, DP, 1>(tile, sub, lane, b, c);
+  return c[0];
+}
+
+// the bf16 column operand of two 16-row steps from an accumulator
+__device__ __forceinline__ void pack_p(const f32x16& p, bf16x8 (&b)[2]) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[m][j] = (bf16_t)p[8 * m + j];
 }
 
 // acc[t] += tile^T (columns 32 t ...) x p, contracted over the tile's rows 32 sub .. 32 sub + 31
+template <int DP>
+__device__ __forceinline__ void cols_mma_packed(const char* tile, int sub, int lane, const bf16x8 (&p)[2],
+                                                f32x16 (&acc)[Tile<bf16_t, DP>::ND]) {
+  const ColReader<DP> rd(tile, lane);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < Tile<bf16_t, DP>::ND; ++t)
+      acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rd.read(sub, m, t), p[m], acc[t], 0, 0, 0);
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void cols_mma(const char* tile, int sub, int lane, const f32x16& p,
                                          f32x16 (&acc)[Tile<T, DP>::ND]) {
   using TL = Tile<T, DP>;
   const int h = lane >> 5;
   if constexpr (sizeof(T) == 2) {
-    const int q4 = (lane & 15) >> 2, p4 = lane & 3, dg = (lane >> 4) & 1;
-    const int r = 4 * h + q4;   // row & 7 of every row this lane addresses
-    const int f = TL::swz(r);
-    const char* base = tile + (32 * sub + r) * TL::RB + (p4 & 1) * 8;
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      bf16x8 b;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) b[j] = (bf16_t)p[8 * m + j];
-#pragma unroll
-      for (int t = 0; t < TL::ND; ++t) {
-        const char* at = base + 16 * m * TL::RB + (((4 * t + 2 * dg + (p4 >> 1)) ^ f) << 4);
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
-        const s16x4 hi =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 8 * TL::RB));
-        typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), b, acc[t], 0, 0, 0);
-      }
-    }
+    bf16x8 b[2];
+    pack_p(p, b);
+    cols_mma_packed<DP>(tile, sub, lane, b, acc);
   } else {
     const int c = (lane & 31) >> 2, w = (lane & 3) * 4;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int row = 8 * (i / 4) + 4 * h + (i & 3);
-      const char* base = tile + (32 * sub + row) * TL::RB + w;
+      const char* base = tile + TL::bytes(32) * sub + TL::off(row) + w;
       const int f = TL::swz(row);
 #pragma unroll
       for (int t = 0; t < TL::ND; ++t) {
@@ -194,31 +234,33 @@ __device__ __forceinline__ void stage(const i32x4& rsrc, char* tile, int dim, OF
     const int slot = it * NT + threadIdx.x;
     const int row = slot / TL::CPR, c = (slot % TL::CPR) ^ TL::swz(row);
     const int o = off(row);
-    dma16(rsrc, tile + (it * NT + wave * 64) * 16, o >= 0 && c * TL::VN < dim ? o + c * 16 : OOB);
+    dma16(rsrc, tile + (it * (NT / 64) + wave) * TL::GS, o >= 0 && c * TL::VN < dim ? o + c * 16 : OOB);
   }
 }
 
 // ROWS rows, stride bytes apart, of which the first `valid` exist: one lane offset serves every pass (the
-// rows of two passes are a multiple of 8 apart, so a chunk's place is the same), the passes advance
+// rows of two passes are a whole period of swz apart, so a chunk's place is the same), the passes advance
 // the descriptor's base, and its length ends with the last row. lane_off(): that offset.
-template <typename T, int DP>
+template <typename T, int DP, int THREADS = NT>
 __device__ __forceinline__ int lane_off(int stride, int dim) {
   using TL = Tile<T, DP>;
-  static_assert(NT / TL::CPR % 8 == 0, "whole swizzle periods a pass");
-  const int row = threadIdx.x / TL::CPR, c = (threadIdx.x % TL::CPR) ^ TL::swz(row);
+  static_assert(THREADS / TL::CPR % TL::PERIOD == 0, "whole periods of swz a pass");
+  const int t = THREADS == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int row = t / TL::CPR, c = (t % TL::CPR) ^ TL::swz(row);
   return c * TL::VN < dim ? row * stride + c * 16 : OOB;
 }
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int THREADS = NT>
 __device__ __forceinline__ void stage_rows(const T* base, int stride, int valid, char* tile, int dim, int off,
                                            int wave) {
   using TL = Tile<T, DP>;
-  constexpr int RPP = NT / TL::CPR;   // rows of a pass
+  constexpr int RPP = THREADS / TL::CPR;   // rows of a pass
+  static_assert(ROWS % RPP == 0, "whole passes");
   const int end = (min(valid, ROWS) - 1) * stride + dim * (int)sizeof(T);   // below 2^31: stride < 2^24
 #pragma unroll
   for (int it = 0; it < ROWS / RPP; ++it) {
     i32x4 r = make_rsrc(reinterpret_cast<const char*>(base) + (int64_t)it * RPP * stride);
     r[2] = max(end - it * RPP * stride, 0);
-    dma16(r, tile + (it * NT + wave * 64) * 16, off);
+    dma16(r, tile + (it * (THREADS / 64) + wave) * TL::GS, off);
   }
 }
 
@@ -258,7 +300,10 @@ struct Item { int b, sub, start, len; };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// cu's sequences, sequence b counting items(b, its length) blocks; it.sub: which of them idx is
+// cu's sequences, sequence b counting items(b, its length, walk) blocks and setting how far each of them
+// walks; it.sub: which of them idx is. Of up to 64 sequences those with longer walks come later (blocks are
+// handed out from the last idx on, so that the longest start first: a 4096-key prompt in front of
+// shorter ones 225 -> 214 us); more stay in order.
 template <typename COUNT>
 __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total, bool tail, int idx, COUNT items,
                                           Item& it) {
@@ -272,19 +317,30 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total
       start = b ? clampi(cu[b], 0, total) : 0;
       len = max(0, (b < nseq ? clampi(cu[b + 1], 0, total) : total) - start);
     }
-    const int cnt = len ? items(b, len) : 0;
-    int inc = cnt;
+    int walk = 0;
+    const int cnt = len ? items(b, len, walk) : 0;
+    int from = 0, all = 0;   // items in front of this lane's, and of all lanes
+    if (n <= 64) {
+      for (int o = 0; o < n; ++o) {
+        const int ow = __builtin_amdgcn_readlane(walk, o), oc = __builtin_amdgcn_readlane(cnt, o);
+        from += ow < walk || (ow == walk && o < lane) ? oc : 0;
+        all += oc;
+      }
+    } else {
+      int inc = cnt;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(inc, o, 64);
-      if (lane >= o) inc += u;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += u;
+      }
+      from = inc - cnt;
+      all = __shfl(inc, 63, 64);
     }
-    const int all = __shfl(inc, 63, 64);
     if (idx < before + all) {
-      const unsigned long long m = __ballot(idx < before + inc);
+      const unsigned long long m = __ballot(idx - before >= from && idx - before < from + cnt);
       const int l = __ffsll((long long)m) - 1;
       it.b = __builtin_amdgcn_readfirstlane(base + l);
-      it.sub = __builtin_amdgcn_readfirstlane(idx - before - __shfl(inc - cnt, l, 64));
+      it.sub = __builtin_amdgcn_readfirstlane(idx - before - __shfl(from, l, 64));
       it.start = __builtin_amdgcn_readfirstlane(__shfl(start, l, 64));
       it.len = __builtin_amdgcn_readfirstlane(__shfl(len, l, 64));
       return true;
@@ -330,18 +386,18 @@ static inline int bias_lds(const Args& a) {
   return a.bias ? a.group * a.buckets * 4 + ((a.nedge ? a.edge[a.nedge - 1] : 0) + 1 + 15) / 16 * 16 : 0;
 }
 
-template <typename T>
+template <typename T, int THREADS = NT>
 __device__ __forceinline__ Bias bias_setup(const Args& a, char* lds, int kvh) {
   float* tab = reinterpret_cast<float*>(lds);
   uint8_t* lut = reinterpret_cast<uint8_t*>(tab + a.group * a.buckets);
   const int heads = a.hkv * a.group;
-  for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) {
+  for (int i = threadIdx.x; i < a.group * a.buckets; i += THREADS) {
     const int g = i / a.buckets, b = i - g * a.buckets;
     const int64_t at = (int64_t)b * heads + kvh * a.group + g;
     tab[i] = a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[at] : to_f32(reinterpret_cast<const T*>(a.bias)[at]);
   }
   const int last = a.nedge ? a.edge[a.nedge - 1] : 0;
-  for (int n = threadIdx.x; n <= last; n += NT) {
+  for (int n = threadIdx.x; n <= last; n += THREADS) {
     int b = 0;
     for (int e = 0; e < a.nedge; ++e) b += a.edge[e] <= n;
     lut[n] = (uint8_t)b;

@@ -25,7 +25,7 @@ using namespace dppa;
 template <typename T, int DP, int WK, int BN, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_bwd_q_kernel(const Args a) {
   using TL = Tile<T, DP>;
-  constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
+  constexpr int TB = TL::bytes(BN), NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
   static_assert(WK == 1 || 4 * TB >= 4 * 32 * OP * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -35,7 +35,11 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   const int heads = a.hkv * a.group;
   float* part = BIAS ? a.dbias_part + ((int64_t)tile * a.hkv + kvh) * a.group * a.buckets : nullptr;
   Item it;
-  if (!find_item(a.cu_q, a.nseq, a.tq, true, tile, [&](int, int len) { return (len * a.group + ROWS - 1) / ROWS; }, it)) {
+  if (!find_item(a.cu_q, a.nseq, a.tq, true, tile,
+                 [&](int b, int len, int& walk) {
+                   walk = seq_at(a.cu_k, a.nseq, a.tk, b).y;
+                   return (len * a.group + ROWS - 1) / ROWS;
+                 }, it)) {
     if constexpr (BIAS)
       for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) part[i] = 0.f;
     return;
@@ -242,7 +246,7 @@ __device__ __forceinline__ int cut_step(int rows, int cuts) { return ((rows + cu
 template <typename T, int DP, int BR, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kernel(const Args a) {
   using TL = Tile<T, DP>;
-  constexpr int TB = BR * TL::RB, NS = BR / 32;
+  constexpr int TB = TL::bytes(BR), NS = BR / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // per row of a tile: lse, D, and (for the bias) its position and head; two buffers, written a tile ahead
   float* lse_s = reinterpret_cast<float*>(smem + 4 * TB);
@@ -256,8 +260,9 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   auto tiles_of = [&](int len) { return (len + BM - 1) / BM; };
   Item it;
   if (!find_item(a.cu_k, a.nseq, a.tk, true, blockIdx.x / a.hkv,
-                 [&](int b, int len) {
-                   return tiles_of(len) * cuts_of(a, seq_at(a.cu_q, a.nseq, a.tq, b).y * a.group);
+                 [&](int b, int len, int& walk) {
+                   walk = seq_at(a.cu_q, a.nseq, a.tq, b).y * a.group;
+                   return tiles_of(len) * cuts_of(a, walk);
                  }, it))
     return;
   const int k0 = it.start, lk = it.len;
@@ -464,7 +469,7 @@ static Plan plan_of(const dp_packed_attn* d) {
   if (wide < 256 && d->tk <= 2048 * seqs) p.wk = d->dtype == DP_F32 && d->dim > 64 ? 2 : 4;
   // the bins beside the waves' larger key tile: where both do not fit the LDS, the waves lie along the rows
   const int dp = d->dim <= 32 ? 32 : d->dim <= 64 ? 64 : 128, last = d->bias && d->buckets > 2 ? 4096 + 16 : 16;
-  if (d->bias && 4 * 32 * p.wk * dp * (d->dtype == DP_F32 ? 4 : 2) + d->buckets * (NT + (int)group) * 4 + last > 163840) p.wk = 1;
+  if (d->bias && 4 * 32 * p.wk * dp * (d->dtype == DP_F32 ? 4 : 2) / 1024 * 1040 + d->buckets * (NT + (int)group) * 4 + last > 163840) p.wk = 1;
   p.items = (int)(rows / (BM / p.wk) + d->nseq + 1);
   // a block of keys walks all rows that see them: the longest such walk bounds the time unless it is
   // cut. About 1024 blocks (causal order leaves half of the cuts empty), at least 512 rows each
@@ -493,7 +498,7 @@ static int grow_lds(const void* kern, int lds) {
 template <typename T, int DP, int WK, bool BIAS>
 int launch_q(const Args& a, hipStream_t s) {
   constexpr int BN = WK > 1 ? 32 * WK : sizeof(T) == 2 ? 64 : 32;
-  const int lds = 4 * BN * Tile<T, DP>::RB + (BIAS ? a.buckets * NT * 4 + bias_lds(a) : 0);
+  const int lds = 4 * Tile<T, DP>::bytes(BN) + (BIAS ? a.buckets * NT * 4 + bias_lds(a) : 0);
   const auto kern = packed_bwd_q_kernel<T, DP, WK, BN, BIAS>;
   if (const int rc = grow_lds((const void*)kern, lds)) return rc;
   hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a);
@@ -507,7 +512,7 @@ int launch(const Args& a, int wk, void* dbias, int bias_f32, hipStream_t s) {
   if (a.tq > 0)
     if (const int rc = wk > 1 ? launch_q<T, DP, W, BIAS>(a, s) : launch_q<T, DP, 1, BIAS>(a, s)) return rc;
   if (a.tk > 0) {
-    const int lds = 4 * BR * Tile<T, DP>::RB + 16 * BR * 2 + bias_lds(a);
+    const int lds = 4 * Tile<T, DP>::bytes(BR) + 16 * BR * 2 + bias_lds(a);
     const auto kern = packed_bwd_kv_kernel<T, DP, BR, BIAS>;
     if (const int rc = grow_lds((const void*)kern, lds)) return rc;
     hipLaunchKernelGGL(kern, dim3(a.ktiles * a.hkv), dim3(NT), lds, s, a);

@@ -60,7 +60,10 @@ __device__ __forceinline__ int splits_of(const Args& a, int lk, int rows) {
 template <typename T, int DP, int WK, int BN, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_fwd_kernel(const Args a, int fill_tail) {
   using TL = Tile<T, DP>;
-  constexpr int TB = BN * TL::RB, NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
+  constexpr int TB = TL::bytes(BN), NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
+  // waves that lie along the keys load what they read themselves and wait for no other
+  constexpr bool OWN = WK == 4 && 64 / TL::CPR % TL::PERIOD == 0;
+  constexpr int SB = TL::bytes(32 * NS);   // a wave's part of a tile
   static_assert(WK == 1 || 4 * TB >= (4 * 32 * (OP + 2) + 2 * ROWS) * 4, "the join of the waves fits the tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -72,7 +75,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   Item it;
   // the last tiles first: in causal order they have the most keys
   if (!find_item(a.cu_q, a.nseq, a.tq, fill_tail || a.splits > 1, a.tiles - 1 - blockIdx.x / a.hkv,
-                 [&](int b, int len) { return tiles_of(len) * cuts_of(len, seq_at(a.cu_k, a.nseq, a.tk, b).y); }, it))
+                 [&](int b, int len, int& walk) {
+                   walk = seq_at(a.cu_k, a.nseq, a.tk, b).y;
+                   return tiles_of(len) * cuts_of(len, walk);
+                 }, it))
     return;
   const int q0 = it.start, lq = it.len;
   int k0, lk;
@@ -100,14 +106,17 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   load_frags<T, DP>((const T*)a.q + (int64_t)(q0 + pos) * a.q_row + (kvh * a.group + g) * a.q_head, ok, a.dim, h, qf);
 
   const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
-  const int koff = lane_off<T, DP>(ks, a.dim), voff = lane_off<T, DP>(vs, a.dim);
+  constexpr int LT = OWN ? 64 : NT;   // threads that load together
+  const int koff = lane_off<T, DP, LT>(ks, a.dim), voff = lane_off<T, DP, LT>(vs, a.dim);
   auto fetch = [&](int j) {
-    char* buf = smem + (j & 1) * 2 * TB;
-    const int key0 = kbeg + j * BN, left = lk - key0;
-    stage_rows<T, DP, BN>((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head, ks, left, buf, a.dim, koff,
-                          wave);
-    stage_rows<T, DP, BN>((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head, vs, left, buf + TB, a.dim,
-                          voff, wave);
+    char* buf = smem + (j & 1) * 2 * TB + (OWN ? wk * SB : 0);
+    const int key0 = kbeg + j * BN + (OWN ? 32 * NS * wk : 0), left = lk - key0;
+    if (OWN && left <= 0) return;
+    constexpr int R = OWN ? 32 * NS : BN;
+    stage_rows<T, DP, R, LT>((const T*)a.k + (int64_t)(k0 + key0) * a.k_row + kvh * a.k_head, ks, left, buf, a.dim, koff,
+                             OWN ? 0 : wave);
+    stage_rows<T, DP, R, LT>((const T*)a.v + (int64_t)(k0 + key0) * a.v_row + kvh * a.v_head, vs, left, buf + TB, a.dim,
+                             voff, OWN ? 0 : wave);
   };
 
   // scores in units in which exp(s - m) = exp2((s - m) c): raw products, or, with a bias, scaled ones
@@ -119,7 +128,12 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
 
   if (nt > 0) fetch(0);
   for (int j = 0; j < nt; ++j) {
-    tile_barrier();
+    if constexpr (OWN) {
+      dpconv::wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+    } else {
+      tile_barrier();
+    }
     if (j + 1 < nt) fetch(j + 1);
     const char* buf = smem + (j & 1) * 2 * TB;
     const int key0 = kbeg + j * BN + 32 * NS * wk;
@@ -168,16 +182,18 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
         for (int i = 0; i < 16; ++i) o[t][i] *= alpha;
     }
     const float mref = m == -INFINITY ? 0.f : m, mc = mref * c;
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         // with a bias s may be the type's lowest value, whose product with c overflows: subtract first
         s[u][i] = __builtin_amdgcn_exp2f(BIAS ? (s[u][i] - mref) * c : fmaf(s[u][i], c, -mc));
-        l += s[u][i];
+        sum[i & 1] += s[u][i];
       }
       cols_mma<T, DP>(buf + TB, NS * wk + u, lane, s[u], o);
     }
+    l += sum[0] + sum[1];
   }
   l = half_sum(l);
 
@@ -299,6 +315,26 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   }
 }
 
+// slow_row of a row of the packed queries (its sequence is searched)
+template <typename T>
+__device__ __forceinline__ void redo_row(const Args& a, int row, int head) {
+  int b = 0;
+  while (b < a.nseq && clampi(a.cu_q[b + 1], 0, a.tq) <= row) ++b;
+  if (b == a.nseq) return;
+  const int2 qs = seq_at(a.cu_q, a.nseq, a.tq, b), ks = seq_at(a.cu_k, a.nseq, a.tk, b);
+  const int pos = row - qs.x, off = ks.y - qs.y;
+  slow_row<T>(a, head / a.group, head % a.group, pos, qs.x, ks.x, a.causal ? clampi(pos + off + 1, 0, ks.y) : ks.y,
+              [&](int j) {
+                if (!a.bias) return 0.f;
+                const int rel = j - pos - off, n = a.both ? abs(rel) : max(-rel, 0);
+                int bk = a.both && rel > 0 ? a.buckets / 2 : 0;
+                for (int e = 0; e < a.nedge; ++e) bk += a.edge[e] <= n;
+                const int64_t x = (int64_t)bk * a.hkv * a.group + head;
+                return a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[x]
+                                  : to_f32(reinterpret_cast<const T*>(a.bias)[x]);
+              });
+}
+
 // rows whose keys were cut: out = sum of the parts weighted by exp(lse - the largest), four elements
 // a thread, in the order of the cuts
 template <typename T, int DP, bool BIAS>
@@ -351,23 +387,57 @@ __global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
     const bool mine = lane / TPR == rr;
     if (!__ballot(bad && mine)) continue;
     const int64_t row_at = (int64_t)blockIdx.x * (NT / TPR) + (threadIdx.x >> 6) * (64 / TPR) + rr;
-    const int row = (int)(row_at / heads), head = (int)(row_at - (int64_t)row * heads);
-    int b = 0;
-    while (b < a.nseq && clampi(a.cu_q[b + 1], 0, a.tq) <= row) ++b;
-    if (b == a.nseq) continue;
-    const int2 qs = seq_at(a.cu_q, a.nseq, a.tq, b), ks = seq_at(a.cu_k, a.nseq, a.tk, b);
-    const int pos = row - qs.x, off = ks.y - qs.y;
-    slow_row<T>(a, head / a.group, head % a.group, pos, qs.x, ks.x, a.causal ? clampi(pos + off + 1, 0, ks.y) : ks.y,
-                [&](int j) {
-                  if (!BIAS) return 0.f;
-                  const int rel = j - pos - off, n = a.both ? abs(rel) : max(-rel, 0);
-                  int bk = a.both && rel > 0 ? a.buckets / 2 : 0;
-                  for (int e = 0; e < a.nedge; ++e) bk += a.edge[e] <= n;
-                  const int64_t x = (int64_t)bk * heads + head;
-                  return a.bias_f32 ? reinterpret_cast<const float*>(a.bias)[x]
-                                    : to_f32(reinterpret_cast<const T*>(a.bias)[x]);
-                });
+    const int row = (int)(row_at / heads);
+    redo_row<T>(a, row, (int)(row_at - (int64_t)row * heads));
   }
+}
+
+// The same for few rows of many parts (single tokens over long caches): a block per row, DP / 4 lanes a
+// part, and the block's 256 / (DP / 4) groups of lanes take parts in turn; summed in a fixed order.
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(NT) void packed_join_row_kernel(const Args a) {
+  constexpr int TPR = DP / 4, GROUPS = NT / TPR;
+  __shared__ f32x4 sm[NT];
+  const int heads = a.hkv * a.group, lane = threadIdx.x & 63;
+  const int64_t all = (int64_t)a.tq * heads, at = blockIdx.x;
+  const int n = uniform(min(a.part_n[at], a.splits));
+  if (n <= 1) return;
+  const float x = lane < n ? a.part_lse[lane * all + at] : -INFINITY;
+  const float top = wave_max(x), ref = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f((x - ref) * (BIAS ? LOG2E : 1.f)), tot = wave_sum(f);
+  const int grp = threadIdx.x / TPR, d = (threadIdx.x % TPR) * 4;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = grp; i < (n + GROUPS - 1) / GROUPS * GROUPS; i += GROUPS) {
+    const float w = __shfl(f, i & 63, 64);   // 0 past the parts
+    if (i < n && d < a.dim) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + (i * all + at) * a.dim + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = fmaf(v[e], w, sum[e]);
+    }
+  }
+  sm[threadIdx.x] = sum;
+  __syncthreads();
+  const float inv = tot == 0.f ? 0.f : 1.f / tot;
+  bool bad = tot != tot;
+  const int row = (int)(at / heads), head = (int)(at - (int64_t)row * heads);
+  if (threadIdx.x < TPR && d < a.dim) {
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += sm[k * TPR + threadIdx.x][e];
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      sum[e] *= inv;
+      bad |= sum[e] != sum[e];
+      w[e] = from_f32<T>(sum[e]);
+    }
+    *reinterpret_cast<T4*>((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d) = w;
+    if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : ref + (BIAS ? __logf(tot) : __log2f(tot));
+  }
+  if (threadIdx.x < 64 && __ballot(bad)) redo_row<T>(a, row, head);
 }
 
 // Which shape a call runs in. Lengths are on the device, so the rule goes by totals.
@@ -404,7 +474,7 @@ static Plan plan_of(const dp_packed_attn* d) {
 template <typename T, int DP, int WK, bool BIAS>
 int launch(const Args& a, int fill_tail, hipStream_t s) {
   constexpr int BN = WK > 1 ? 32 * WK : sizeof(T) == 2 ? 64 : 32;
-  const int lds = 4 * BN * Tile<T, DP>::RB + bias_lds(a);
+  const int lds = 4 * Tile<T, DP>::bytes(BN) + bias_lds(a);
   const auto kern = packed_fwd_kernel<T, DP, WK, BN, BIAS>;
   if (lds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -413,7 +483,10 @@ int launch(const Args& a, int fill_tail, hipStream_t s) {
   hipLaunchKernelGGL(kern, dim3(a.tiles * a.hkv), dim3(NT), lds, s, a, fill_tail);
   if (a.splits > 1) {
     const int64_t n = (int64_t)a.tq * a.hkv * a.group, per = NT / (DP / 4);
-    hipLaunchKernelGGL((packed_join_kernel<T, DP, BIAS>), dim3((unsigned)((n + per - 1) / per)), dim3(NT), 0, s, a);
+    if (n <= 4096)
+      hipLaunchKernelGGL((packed_join_row_kernel<T, DP, BIAS>), dim3((unsigned)n), dim3(NT), 0, s, a);
+    else
+      hipLaunchKernelGGL((packed_join_kernel<T, DP, BIAS>), dim3((unsigned)((n + per - 1) / per)), dim3(NT), 0, s, a);
   }
   return dp_check_launch("dp_packed_attn_fwd");
 }
