@@ -296,29 +296,32 @@ __device__ __forceinline__ void tile_barrier() {
 // The lengths are on the device only: a launch has as many blocks as the packed total allows at
 // most, and every wave finds its block's (sequence, tile) by a scan over the sequences, 64 at a time.
 // nseq counts one more when the rows behind the last sequence are an item of their own (tail).
-struct Item { int b, sub, start, len; };
+struct Item { int b, sub, start, len, start2, len2; };   // start2, len2: of the other side's rows
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// cu's sequences, sequence b counting items(b, its length, walk) blocks and setting how far each of them
-// walks; it.sub: which of them idx is. Of up to 64 sequences those with longer walks come later (blocks are
+// cu's sequences, a sequence counting items(its length, its length by cu2) blocks, each of which walks that second
+// length; it.sub: which of them idx is. Of up to 64 sequences those with longer walks come later (blocks are
 // handed out from the last idx on, so that the longest start first: a 4096-key prompt in front of
 // shorter ones 225 -> 214 us); more stay in order.
 template <typename COUNT>
-__device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total, bool tail, int idx, COUNT items,
-                                          Item& it) {
+__device__ __forceinline__ bool find_item(const int32_t* cu, int total, const int32_t* cu2, int total2, int nseq,
+                                          bool tail, int idx, COUNT items, Item& it) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   const int n = nseq + (tail ? 1 : 0);
   for (int base = 0; base < n; base += 64) {
     const int b = base + lane;
-    int start = 0, len = 0;
+    int start = 0, len = 0, start2 = 0, walk = 0;
     if (b < n) {
-      start = b ? clampi(cu[b], 0, total) : 0;
-      len = max(0, (b < nseq ? clampi(cu[b + 1], 0, total) : total) - start);
+      // all four at once: a small call's time is the number of round trips
+      const int c0 = cu[min(b, nseq)], c1 = cu[min(b + 1, nseq)], d0 = cu2[min(b, nseq)], d1 = cu2[min(b + 1, nseq)];
+      start = b ? clampi(c0, 0, total) : 0;
+      len = max(0, (b < nseq ? clampi(c1, 0, total) : total) - start);
+      start2 = b && b < nseq ? clampi(d0, 0, total2) : 0;
+      walk = b < nseq ? max(0, clampi(d1, 0, total2) - start2) : 0;
     }
-    int walk = 0;
-    const int cnt = len ? items(b, len, walk) : 0;
+    const int cnt = len ? items(len, walk) : 0;
     int from = 0, all = 0;   // items in front of this lane's, and of all lanes
     if (n <= 64) {
       for (int o = 0; o < n; ++o) {
@@ -343,6 +346,8 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int nseq, int total
       it.sub = __builtin_amdgcn_readfirstlane(idx - before - __shfl(from, l, 64));
       it.start = __builtin_amdgcn_readfirstlane(__shfl(start, l, 64));
       it.len = __builtin_amdgcn_readfirstlane(__shfl(len, l, 64));
+      it.start2 = __builtin_amdgcn_readfirstlane(__shfl(start2, l, 64));
+      it.len2 = __builtin_amdgcn_readfirstlane(__shfl(walk, l, 64));
       return true;
     }
     before += all;
@@ -355,14 +360,6 @@ __device__ __forceinline__ int2 seq_at(const int32_t* cu, int nseq, int total, i
   const int start = b && b < nseq ? clampi(cu[b], 0, total) : 0;
   return int2{start, b < nseq ? max(0, clampi(cu[b + 1], 0, total) - start) : 0};
 }
-__device__ __forceinline__ void seq_of(const int32_t* cu, int nseq, int total, int b, int& start, int& len) {
-  const int2 s = seq_at(cu, nseq, total, b);
-  start = s.x;
-  len = s.y;
-  start = __builtin_amdgcn_readfirstlane(start);
-  len = __builtin_amdgcn_readfirstlane(len);
-}
-
 // ---------------------------------------------------------------- relative position bias
 // LDS: tab[g][bucket] f32 of the group's heads, then lut[n] = bucket of distance n, n <= last (the
 // distance from which on every one is in the last bucket).

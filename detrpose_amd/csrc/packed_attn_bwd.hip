@@ -35,18 +35,13 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   const int heads = a.hkv * a.group;
   float* part = BIAS ? a.dbias_part + ((int64_t)tile * a.hkv + kvh) * a.group * a.buckets : nullptr;
   Item it;
-  if (!find_item(a.cu_q, a.nseq, a.tq, true, tile,
-                 [&](int b, int len, int& walk) {
-                   walk = seq_at(a.cu_k, a.nseq, a.tk, b).y;
-                   return (len * a.group + ROWS - 1) / ROWS;
-                 }, it)) {
+  if (!find_item(a.cu_q, a.tq, a.cu_k, a.tk, a.nseq, true, tile,
+                 [&](int len, int) { return (len * a.group + ROWS - 1) / ROWS; }, it)) {
     if constexpr (BIAS)
       for (int i = threadIdx.x; i < a.group * a.buckets; i += NT) part[i] = 0.f;
     return;
   }
-  const int q0 = it.start, lq = it.len;
-  int k0, lk;
-  seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
+  const int q0 = it.start, lq = it.len, k0 = it.start2, lk = it.len2;
   const int off = lk - lq, rows = lq * a.group, row0 = it.sub * ROWS;
   const int first = row0 + 32 * wr, r = first + (lane & 31);
   const bool ok = r < rows;
@@ -259,15 +254,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   const int heads = a.hkv * a.group;
   auto tiles_of = [&](int len) { return (len + BM - 1) / BM; };
   Item it;
-  if (!find_item(a.cu_k, a.nseq, a.tk, true, blockIdx.x / a.hkv,
-                 [&](int b, int len, int& walk) {
-                   walk = seq_at(a.cu_q, a.nseq, a.tq, b).y * a.group;
-                   return tiles_of(len) * cuts_of(a, walk);
-                 }, it))
+  if (!find_item(a.cu_k, a.tk, a.cu_q, a.tq, a.nseq, true, blockIdx.x / a.hkv,
+                 [&](int len, int queries) { return tiles_of(len) * cuts_of(a, queries * a.group); }, it))
     return;
-  const int k0 = it.start, lk = it.len;
-  int q0, lq;
-  seq_of(a.cu_q, a.nseq, a.tq, it.b, q0, lq);
+  const int k0 = it.start, lk = it.len, q0 = it.start2, lq = it.len2;
   const int off = lk - lq, rows = lq * a.group, ntile = tiles_of(lk);
   const int cuts = uniform(cuts_of(a, rows)), cut = uniform(it.sub / ntile), tile = it.sub - cut * ntile;
   const int first = tile * BM + 32 * wave, key = first + (lane & 31);

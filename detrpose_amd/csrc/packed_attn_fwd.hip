@@ -74,15 +74,10 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
   auto cuts_of = [&](int lq, int lk) { return splits_of(a, lk, min(ROWS, lq * a.group)); };
   Item it;
   // the last tiles first: in causal order they have the most keys
-  if (!find_item(a.cu_q, a.nseq, a.tq, fill_tail || a.splits > 1, a.tiles - 1 - blockIdx.x / a.hkv,
-                 [&](int b, int len, int& walk) {
-                   walk = seq_at(a.cu_k, a.nseq, a.tk, b).y;
-                   return tiles_of(len) * cuts_of(len, walk);
-                 }, it))
+  if (!find_item(a.cu_q, a.tq, a.cu_k, a.tk, a.nseq, fill_tail || a.splits > 1, a.tiles - 1 - blockIdx.x / a.hkv,
+                 [&](int len, int keys) { return tiles_of(len) * cuts_of(len, keys); }, it))
     return;
-  const int q0 = it.start, lq = it.len;
-  int k0, lk;
-  seq_of(a.cu_k, a.nseq, a.tk, it.b, k0, lk);
+  const int q0 = it.start, lq = it.len, k0 = it.start2, lk = it.len2;
   const int cuts = uniform(cuts_of(lq, lk)), ntile = uniform(tiles_of(lq)), cut = uniform(it.sub / ntile);
   const int off = lk - lq, rows = lq * a.group, row0 = (it.sub - cut * ntile) * ROWS;
   const int first = row0 + 32 * wr, r = first + (lane & 31);
@@ -451,9 +446,10 @@ static Plan plan_of(const dp_packed_attn* d) {
   const int per = BM / p.wk;
   int64_t items = rows / per + d->nseq + 1;
   if (d->tk > 1024 && (few || (rows / per + 1) * d->kv_heads < 256) && d->tq > 0) {
-    // about 1024 blocks of few rows, or 512 of many; a part of the output is written in f32 per cut and row, so a
-    // cut has at least 16 keys a row (splits_of)
-    const int64_t target = few ? 1024 : 512;
+    // about 256 blocks of few rows (a block's start costs as much as 20 tiles: 64 sequences of 2000 keys 80 us with
+    // 1024 blocks, 62 with 512, 57 with 256; 131 k ragged keys 139, 130, 133), or 512 of many; a part of the output
+    // is written in f32 per cut and row, so a cut has at least 16 keys a row (splits_of)
+    const int64_t target = few ? 256 : 512;
     const int64_t most_tiles = rows / per + 1;             // of one sequence
     int64_t chunk = std::max<int64_t>(256, (int64_t)d->tk * d->kv_heads * (few ? 1 : (items + seqs) / seqs) / target);
     chunk = (chunk + 127) / 128 * 128;
