@@ -24,7 +24,6 @@
 
 namespace dppa {
 
-using dpconv::dma16;
 using dpconv::i32x4;
 using dpconv::make_rsrc;
 using dpconv::OOB;
@@ -61,10 +60,47 @@ struct Args {
   void *dq, *dk, *dv;
   float* dsum;
   float* dbias_part;
-  int ktiles, cut_rows, cuts;   // dk / dv: blocks, rows of a cut at least, most cuts of one sequence
+  int ktiles, cut_tiles, cuts;   // dk / dv: blocks, query tiles of a cut, most cuts of one sequence
   float* kv_part;
   int* kv_n;
 };
+
+// A wave-uniform value in a scalar register (the empty asm keeps it there: the compiler drops a
+// readfirstlane of what it knows to be uniform and may then carry on with vector instructions)
+__device__ __forceinline__ int uniform(int x) {
+  x = __builtin_amdgcn_readfirstlane(x);
+  asm("" : "+s"(x));
+  return x;
+}
+
+// 16 bytes a lane from rsrc + off (zero outside) to LDS, lane L at at + 16 L; 4 bytes a lane for the first n
+// lanes. A FRESH descriptor may just have been written by vector instructions (readfirstlane), which a memory
+// instruction may read 5 wait states later, and m0 one after its write: the nop counts these, as the
+// compiler does not look into the asm. Completion is waited for by hand.
+template <bool FRESH = true>
+__device__ __forceinline__ void dma16(const i32x4& rsrc, const char* at, int off, int soff = 0) {
+  const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(at));
+  i32x4 r;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) r[w] = __builtin_amdgcn_readfirstlane(rsrc[w]);
+  if (FRESH)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(off), "s"(r),
+                 "s"(soff)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(off), "s"(r),
+                 "s"(soff)
+                 : "memory");
+}
+__device__ __forceinline__ void dma4(const i32x4& rsrc, const char* at, int off, int n) {
+  const unsigned m0 = __builtin_amdgcn_readfirstlane((unsigned)reinterpret_cast<uintptr_t>(at));
+  i32x4 r;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) r[w] = __builtin_amdgcn_readfirstlane(rsrc[w]);
+  if ((int)(threadIdx.x & 63) < n)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r)
+                 : "memory");
+}
 
 template <typename T> struct Tr;
 template <> struct Tr<bf16_t> { static constexpr int VN = 8; };
@@ -223,24 +259,11 @@ __device__ __forceinline__ void cols_mma(const char* tile, int sub, int lane, co
   }
 }
 
-// ROWS rows into a tile: row r from rsrc + off(r) bytes, zero where off is negative or past dim
-template <typename T, int DP, int ROWS, typename OFF>
-__device__ __forceinline__ void stage(const i32x4& rsrc, char* tile, int dim, OFF off) {
-  using TL = Tile<T, DP>;
-  static_assert(ROWS * TL::CPR % NT == 0, "whole passes");
-  const int wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int it = 0; it < ROWS * TL::CPR / NT; ++it) {
-    const int slot = it * NT + threadIdx.x;
-    const int row = slot / TL::CPR, c = (slot % TL::CPR) ^ TL::swz(row);
-    const int o = off(row);
-    dma16(rsrc, tile + (it * (NT / 64) + wave) * TL::GS, o >= 0 && c * TL::VN < dim ? o + c * 16 : OOB);
-  }
-}
-
 // ROWS rows, stride bytes apart, of which the first `valid` exist: one lane offset serves every pass (the
-// rows of two passes are a whole period of swz apart, so a chunk's place is the same), the passes advance
-// the descriptor's base, and its length ends with the last row. lane_off(): that offset.
+// rows of two passes are a whole period of swz apart, so a chunk's place is the same). A whole tile's
+// passes share a descriptor and differ in the scalar offset; the last, partial one moves the descriptor's
+// base instead, whose length ends with the last row (a scalar offset past the length would wrap the
+// hardware's range check). lane_off(): that offset.
 template <typename T, int DP, int THREADS = NT>
 __device__ __forceinline__ int lane_off(int stride, int dim) {
   using TL = Tile<T, DP>;
@@ -255,7 +278,15 @@ __device__ __forceinline__ void stage_rows(const T* base, int stride, int valid,
   using TL = Tile<T, DP>;
   constexpr int RPP = THREADS / TL::CPR;   // rows of a pass
   static_assert(ROWS % RPP == 0, "whole passes");
-  const int end = (min(valid, ROWS) - 1) * stride + dim * (int)sizeof(T);   // below 2^31: stride < 2^24
+  if (valid >= ROWS) {
+    const i32x4 r = make_rsrc(base);
+    dma16(r, tile + wave * TL::GS, off);
+#pragma unroll
+    for (int it = 1; it < ROWS / RPP; ++it)
+      dma16<false>(r, tile + (it * (THREADS / 64) + wave) * TL::GS, off, it * RPP * stride);
+    return;
+  }
+  const int end = (valid - 1) * stride + dim * (int)sizeof(T);   // below 2^31: stride < 2^24
 #pragma unroll
   for (int it = 0; it < ROWS / RPP; ++it) {
     i32x4 r = make_rsrc(reinterpret_cast<const char*>(base) + (int64_t)it * RPP * stride);
@@ -263,8 +294,6 @@ __device__ __forceinline__ void stage_rows(const T* base, int stride, int valid,
     dma16(r, tile + (it * (THREADS / 64) + wave) * TL::GS, off);
   }
 }
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // the lane's fragments of one global row as a B operand (zero when !ok and past dim)
 template <typename T, int DP>
@@ -305,8 +334,8 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x,
 // handed out from the last idx on, so that the longest start first: a 4096-key prompt in front of
 // shorter ones 225 -> 214 us); more stay in order.
 template <typename COUNT>
-__device__ __forceinline__ bool find_item(const int32_t* cu, int total, const int32_t* cu2, int total2, int nseq,
-                                          bool tail, int idx, COUNT items, Item& it) {
+__device__ __forceinline__ bool search_item(const int32_t* cu, int total, const int32_t* cu2, int total2, int nseq,
+                                            bool tail, int idx, COUNT items, Item& it) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   const int n = nseq + (tail ? 1 : 0);
@@ -342,17 +371,27 @@ __device__ __forceinline__ bool find_item(const int32_t* cu, int total, const in
     if (idx < before + all) {
       const unsigned long long m = __ballot(idx - before >= from && idx - before < from + cnt);
       const int l = __ffsll((long long)m) - 1;
-      it.b = __builtin_amdgcn_readfirstlane(base + l);
-      it.sub = __builtin_amdgcn_readfirstlane(idx - before - __shfl(from, l, 64));
-      it.start = __builtin_amdgcn_readfirstlane(__shfl(start, l, 64));
-      it.len = __builtin_amdgcn_readfirstlane(__shfl(len, l, 64));
-      it.start2 = __builtin_amdgcn_readfirstlane(__shfl(start2, l, 64));
-      it.len2 = __builtin_amdgcn_readfirstlane(__shfl(walk, l, 64));
+      it.b = base + l;
+      it.sub = idx - before - __shfl(from, l, 64);
+      it.start = __shfl(start, l, 64);
+      it.len = __shfl(len, l, 64);
+      it.start2 = __shfl(start2, l, 64);
+      it.len2 = __shfl(walk, l, 64);
       return true;
     }
     before += all;
   }
   return false;
+}
+
+template <typename COUNT>
+__device__ __forceinline__ bool find_item(const int32_t* cu, int total, const int32_t* cu2, int total2, int nseq,
+                                          bool tail, int idx, COUNT items, Item& it) {
+  Item x{};
+  const bool found = search_item(cu, total, cu2, total2, nseq, tail, idx, items, x);
+  // made scalar here, behind the search's loop, whose exit the compiler takes for one that lanes leave singly
+  it = Item{uniform(x.b), uniform(x.sub), uniform(x.start), uniform(x.len), uniform(x.start2), uniform(x.len2)};
+  return uniform(found) != 0;
 }
 
 // start and length of sequence b (nothing for the tail)

@@ -5,7 +5,7 @@
 //
 // Two kernels, each owner of what it writes, so nothing is added atomically and equal inputs give
 // equal bits: packed_bwd_q_kernel walks the keys of a tile of 128 rows (S^T, dP^T, dQ^T: three products)
-// and stores D; packed_bwd_kv_kernel walks the rows (all heads of the group, so grouped heads are summed
+// and stores D; packed_bwd_kv_kernel walks the rows (head after head of the group, so grouped heads are summed
 // in the accumulators) of a tile of 128 keys (S, dP, dV^T, dK^T: four products). Two of the seven products
 // are done twice in exchange. p and ds are rounded to bf16 for their products, as p in the forward.
 //
@@ -23,7 +23,8 @@ using namespace dppa;
 
 // WK waves of a block share its rows and take the key tile's subtiles in turn, as in the forward
 template <typename T, int DP, int WK, int BN, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_bwd_q_kernel(const Args a) {
+__global__ __launch_bounds__(NT)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 128 ? 2 : 8))) void packed_bwd_q_kernel(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int TB = TL::bytes(BN), NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
   static_assert(WK == 1 || 4 * TB >= 4 * 32 * OP * 4, "the join of the waves fits the tiles");
@@ -232,95 +233,77 @@ __global__ __launch_bounds__(NT) void packed_dbias_kernel(TB* __restrict__ out, 
     out[(int64_t)b * hkv * group + head] = from_f32<TB>((sm[b] + sm[64 + b]) + (sm[128 + b] + sm[192 + b]));
 }
 
-// rows [cut * step, ...) of a sequence's cuts
-__device__ __forceinline__ int cuts_of(const Args& a, int rows) {
-  return a.cuts <= 1 ? 1 : clampi((rows + a.cut_rows - 1) / a.cut_rows, 1, a.cuts);
+// A block owns 128 keys (32 a wave, their K and V fragments in registers) and walks tiles of BR query rows of one
+// head after the other, all heads of the group: W = group x (query tiles that see its first key) tiles,
+// which are cut into equal runs where one block's walk would outlast the rest.
+__device__ __forceinline__ int cuts_of(const Args& a, int tiles) {
+  return a.cuts <= 1 ? 1 : clampi((tiles + a.cut_tiles - 1) / a.cut_tiles, 1, a.cuts);
 }
-__device__ __forceinline__ int cut_step(int rows, int cuts) { return ((rows + cuts - 1) / cuts + 31) / 32 * 32; }
 
 template <typename T, int DP, int BR, bool BIAS>
 __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kernel(const Args a) {
   using TL = Tile<T, DP>;
   constexpr int TB = TL::bytes(BR), NS = BR / 32;
+  // bf16 at dim 128: dk, dv and the K fragments take 160 of a wave's 256 registers; V's stay in LDS (with
+  // them in registers 11 to 34 spilled, and each reload waited for the tile loads in flight)
+  constexpr bool VL = sizeof(T) == 2 && DP == 128;
+  constexpr int VB = VL ? TL::bytes(BM) : 0;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // per row of a tile: lse, D, and (for the bias) its position and head; two buffers, written a tile ahead
-  float* lse_s = reinterpret_cast<float*>(smem + 4 * TB);
+  char* const vtile = smem + 4 * TB;
+  // lse and D of a tile's rows, two buffers
+  float* lse_s = reinterpret_cast<float*>(vtile + VB);
   float* dsum_s = lse_s + 2 * BR;
-  int* pos_s = reinterpret_cast<int*>(dsum_s + 2 * BR);
-  int* head_s = pos_s + 2 * BR;
   const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // uniform: scalar branches below
+  const int wave = uniform(threadIdx.x >> 6);   // uniform: scalar branches below
   const int kvh = uniform(blockIdx.x % a.hkv);
   const int heads = a.hkv * a.group;
   auto tiles_of = [&](int len) { return (len + BM - 1) / BM; };
   Item it;
   if (!find_item(a.cu_k, a.tk, a.cu_q, a.tq, a.nseq, true, blockIdx.x / a.hkv,
-                 [&](int len, int queries) { return tiles_of(len) * cuts_of(a, queries * a.group); }, it))
+                 [&](int len, int queries) {
+                   return tiles_of(len) * cuts_of(a, (queries + BR - 1) / BR * a.group);
+                 }, it))
     return;
   const int k0 = it.start, lk = it.len, q0 = it.start2, lq = it.len2;
-  const int off = lk - lq, rows = lq * a.group, ntile = tiles_of(lk);
-  const int cuts = uniform(cuts_of(a, rows)), cut = uniform(it.sub / ntile), tile = it.sub - cut * ntile;
+  const int off = lk - lq, ntile = tiles_of(lk), qtiles = (lq + BR - 1) / BR;
+  const int most = uniform(cuts_of(a, qtiles * a.group)), cut = uniform(it.sub / ntile), tile = uniform(it.sub - cut * ntile);
   const int first = tile * BM + 32 * wave, key = first + (lane & 31);
   const bool ok = key < lk;
-  // the first row that sees a key
-  auto sees = [&](int kk) { return a.causal ? max(0, kk - off) * a.group : 0; };
-  const int mine = sees(key), wfirst = uniform(sees(first)), wlast = uniform(sees(min(first + 31, lk - 1)));
-  // this block's rows [start, end)
-  const int seen = sees(tile * BM) / 32 * 32, step = cuts > 1 ? cut_step(rows, cuts) : 0;
-  const int start = uniform(max(seen, cut * step)), end = uniform(cuts > 1 ? min(rows, (cut + 1) * step) : rows);
-  if (start >= end && cuts > 1) return;
+  // the first query that sees a key
+  auto sees = [&](int kk) { return a.causal ? max(0, kk - off) : 0; };
+  const int mine = ok ? sees(key) : lq, wfirst = uniform(sees(first)), wlast = uniform(sees(min(first + 31, lk - 1)));
+  const unsigned seen = (unsigned)max(0, lq - mine);
+  // this block's run of the walk
+  const int from = uniform(min(sees(tile * BM) / BR, qtiles)), nper = qtiles - from, all = nper * a.group;
+  const int cuts = uniform(min(most, cuts_of(a, all))), step = uniform((all + cuts - 1) / cuts);
+  if (cut >= cuts) return;
+  const int w0 = cut * step, w1 = uniform(min(all, w0 + step));
   Bias bias{};
-  if constexpr (BIAS) bias = bias_setup<T>(a, smem + 4 * TB + 16 * BR * 2, kvh);
+  if constexpr (BIAS) bias = bias_setup<T>(a, vtile + VB + 16 * BR, kvh);
 
-  u32x4 kf[TL::KS], vf[TL::KS];
+  u32x4 kf[TL::KS], vf[VL ? 1 : TL::KS];
   load_frags<T, DP>((const T*)a.k + (int64_t)(k0 + min(key, lk - 1)) * a.k_row + kvh * a.k_head, ok, a.dim, h, kf);
-  load_frags<T, DP>((const T*)a.v + (int64_t)(k0 + min(key, lk - 1)) * a.v_row + kvh * a.v_head, ok, a.dim, h, vf);
+  if constexpr (VL) {
+    const int vs = (int)(a.v_row * sizeof(T));
+    stage_rows<T, DP, BM>((const T*)a.v + (int64_t)(k0 + tile * BM) * a.v_row + kvh * a.v_head, vs, lk - tile * BM, vtile,
+                          a.dim, lane_off<T, DP>(vs, a.dim), wave);
+  } else {
+    load_frags<T, DP>((const T*)a.v + (int64_t)(k0 + min(key, lk - 1)) * a.v_row + kvh * a.v_head, ok, a.dim, h, vf);
+  }
 
-  const int nt = end > start ? (end - start + BR - 1) / BR : 0;
-  const float invg = 1.f / (float)a.group;
-  // lse and D of the next tile's rows are loaded with it and stored a step later
-  float lse_r = INFINITY, dsum_r = 0.f;
-  int pos_r = 0, head_r = 0;
-  auto fetch = [&](int j) {
-    char* buf = smem + (j & 1) * 2 * TB;
-    const int r0 = start + j * BR, p0 = r0 / a.group, skip = r0 - p0 * a.group;
-    const i32x4 rq = make_rsrc((const T*)a.q + (int64_t)(q0 + p0) * a.q_row + kvh * a.group * a.q_head);
-    const i32x4 rg = make_rsrc((const T*)a.dout + (int64_t)(q0 + p0) * a.g_row + kvh * a.group * a.g_head);
-    // (query, head) of the tile's row: a small quotient, exact in f32
-    auto split = [&](int row, int& p, int& g) {
-      p = (int)(((float)(skip + row) + 0.5f) * invg);
-      g = skip + row - p * a.group;
-    };
-    auto at = [&](int row, int64_t rs, int64_t hs) {
-      int p, g;
-      split(row, p, g);
-      return r0 + row < end ? p * (int)(rs * sizeof(T)) + g * (int)(hs * sizeof(T)) : -1;
-    };
-    stage<T, DP, BR>(rq, buf, a.dim, [&](int row) { return at(row, a.q_row, a.q_head); });
-    stage<T, DP, BR>(rg, buf + TB, a.dim, [&](int row) { return at(row, a.g_row, a.g_head); });
-    if (threadIdx.x < BR) {
-      lse_r = INFINITY;   // a row past the end: p = 0
-      dsum_r = 0.f;
-      if (r0 + (int)threadIdx.x < end) {
-        int p, g;
-        split(threadIdx.x, p, g);
-        const int64_t x = (int64_t)(q0 + p0 + p) * heads + kvh * a.group + g;
-        lse_r = a.lse[x];
-        dsum_r = a.dsum[x];
-        pos_r = p0 + p;
-        head_r = g;
-      }
-    }
-  };
-  auto publish = [&](int j) {
-    if (threadIdx.x < BR) {
-      const int x = (j & 1) * BR + threadIdx.x;
-      lse_s[x] = lse_r;
-      dsum_s[x] = dsum_r;
-      if constexpr (BIAS) {
-        pos_s[x] = pos_r;
-        head_s[x] = head_r;
-      }
+  const int qs = (int)(a.q_row * sizeof(T)), gs = (int)(a.g_row * sizeof(T));
+  const int qoff = lane_off<T, DP>(qs, a.dim), goff = lane_off<T, DP>(gs, a.dim);
+  auto fetch = [&](int buf, int g, int t) {
+    char* at = smem + buf * 2 * TB;
+    const int p0 = t * BR, left = lq - p0, head = kvh * a.group + g;
+    stage_rows<T, DP, BR>((const T*)a.q + (int64_t)(q0 + p0) * a.q_row + head * a.q_head, qs, left, at, a.dim, qoff, wave);
+    stage_rows<T, DP, BR>((const T*)a.dout + (int64_t)(q0 + p0) * a.g_row + head * a.g_head, gs, left, at + TB, a.dim,
+                          goff, wave);
+    // the first two waves: lse and D, one row a lane (0 past the sequence, where q, dout and p are 0 too)
+    if (wave < 2) {
+      const int64_t x = (int64_t)(q0 + p0) * heads + head;
+      const i32x4 rs = make_rsrc(wave ? a.dsum + x : a.lse + x);
+      dma4(rs, reinterpret_cast<char*>((wave ? dsum_s : lse_s) + buf * BR), lane < min(left, BR) ? lane * heads * 4 : OOB, BR);
     }
   };
 
@@ -329,56 +312,78 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
 #pragma unroll
   for (int t = 0; t < TL::ND; ++t) dk[t] = dv[t] = zero16();
 
-  if (nt > 0) fetch(0);
-  for (int j = 0; j < nt; ++j) {
-    dpconv::wait_vmcnt<0>();
-    publish(j);
-    __syncthreads();
-    if (j + 1 < nt) fetch(j + 1);
-    const char* buf = smem + (j & 1) * 2 * TB;
-    const int r0 = start + j * BR;
+  dpconv::wait_vmcnt<0>();   // the fragments above, so that the loop's waits count tiles only
+  int g = uniform(nper ? w0 / nper : 0), t = uniform(from + w0 - g * nper);
+  if (w0 < w1) fetch(0, g, t);
+  for (int w = w0; w < w1; ++w) {
+    tile_barrier();
+    const int b = (w - w0) & 1, p0 = t * BR, gh = g;
+    const bool turn = t + 1 == qtiles;
+    t = uniform(turn ? from : t + 1);
+    g = uniform(turn ? g + 1 : g);
+    if (w + 1 < w1) fetch(b ^ 1, g, t);
+    const char* buf = smem + b * 2 * TB;
     if (first >= lk) continue;
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
-      const int r32 = r0 + 32 * u;
-      if (r32 >= end) break;
-      if (r32 + 31 < wfirst) continue;
-      const int x0 = (j & 1) * BR + 32 * u + 4 * h;
+      const int p32 = p0 + 32 * u;
+      if (p32 >= lq) break;
+      if (p32 + 31 < wfirst) continue;
       f32x16 s = rows_mma<T, DP>(buf, u, lane, kf);
       if constexpr (BIAS) {
-        const int pf = r32 / a.group + off, pl = min(r32 + 31, rows - 1) / a.group + off;
-        const int one = bias.one_bucket(first - pl, first + 31 - pf);
+        const float* tab = bias.tab + gh * bias.nb;
+        const int rel0 = key - off - p32 - 4 * h;
+        const int one = bias.one_bucket(first - min(p32 + 31, lq - 1) - off, first + 31 - p32 - off);
+        if (one >= 0) {
+          const float x = tab[one];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int x = x0 + 8 * (i / 4) + (i & 3);
-          const int b = one >= 0 ? one : bias.bucket(key - pos_s[x] - off);
-          s[i] = fmaf(s[i], a.scale, bias.tab[head_s[x] * bias.nb + b]);
+          for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], a.scale, x);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], a.scale, tab[bias.bucket(rel0 - 8 * (i / 4) - (i & 3))]);
         }
       }
-      f32x16 p;
+      const int x0 = b * BR + 32 * u + 4 * h;
+      const bool edge = p32 < wlast || p32 + 32 > lq || first + 32 > lk;
+      // queries [mine, lq) see the key: one comparison each
+      auto hidden = [&](int i) { return (unsigned)(p32 + 8 * (i / 4) + 4 * h + (i & 3) - mine) >= seen; };
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + x0 + 8 * e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float v = s[4 * e + i];
-          p[4 * e + i] = __builtin_amdgcn_exp2f(BIAS ? (v - ls[i]) * LOG2E : fmaf(v, c, -ls[i]));
+          s[4 * e + i] = __builtin_amdgcn_exp2f(BIAS ? (v - ls[i]) * LOG2E : fmaf(v, c, -ls[i]));
         }
       }
-      if (r32 < wlast || !ok) {
+      if (edge) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (r32 + 8 * (i / 4) + 4 * h + (i & 3) < mine || !ok) p[i] = 0.f;
+          if (hidden(i)) s[i] = 0.f;
       }
-      cols_mma<T, DP>(buf + TB, u, lane, p, dv);
-      const f32x16 dp = rows_mma<T, DP>(buf + TB, u, lane, vf);
+      cols_mma<T, DP>(buf + TB, u, lane, s, dv);
+      f32x16 dp;
+      if constexpr (VL) {
+        const RowReader<T, DP> gr(buf + TB + TL::bytes(32) * u, lane), vr(vtile + TL::bytes(32) * wave, lane);
+        dp = zero16();
+#pragma unroll
+        for (int q = 0; q < TL::KS; ++q)
+          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gr.read(0, q), vr.read(0, q), dp, 0, 0, 0);
+      } else {
+        dp = rows_mma<T, DP>(buf + TB, u, lane, vf);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const f32x4 ds = *reinterpret_cast<const f32x4*>(dsum_s + x0 + 8 * e);
+        const f32x4 dd = *reinterpret_cast<const f32x4*>(dsum_s + x0 + 8 * e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[4 * e + i] *= dp[4 * e + i] - ds[i];
+        for (int i = 0; i < 4; ++i) s[4 * e + i] *= dp[4 * e + i] - dd[i];
       }
-      cols_mma<T, DP>(buf, u, lane, p, dk);
+      if (edge) {   // dout of a hidden query may be anything
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (hidden(i)) s[i] = 0.f;
+      }
+      cols_mma<T, DP>(buf, u, lane, s, dk);
     }
   }
 
@@ -413,8 +418,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
           }
         }
       }
-    // the last cut's rows see every key: it says which cuts there are (and 0 of them where it wrote the result)
-    if (a.cuts > 1 && cut == cuts - 1 && h == 0) a.kv_n[kr] = cuts > 1 ? (seen / step) << 16 | cuts : 0;
+    if (a.cuts > 1 && cut == 0 && h == 0) a.kv_n[kr] = cuts;   // 1: the result is written
   }
 }
 
@@ -426,11 +430,11 @@ __global__ __launch_bounds__(NT) void packed_kv_join_kernel(const Args a) {
   const int64_t kr = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
   const int d = (threadIdx.x % TPR) * 4;
   if (kr >= all || d >= a.dim) return;
-  const int n = a.kv_n[kr], from = n >> 16, to = min(n & 0xffff, a.cuts);
-  if (n <= 0) return;
+  const int n = min(a.kv_n[kr], a.cuts);
+  if (n <= 1) return;
   f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
 #pragma unroll 4
-  for (int c = from; c < to; ++c) {
+  for (int c = 0; c < n; ++c) {
     const float* part = a.kv_part + (c * all + kr) * 2 * a.dim + d;
     const f32x4 u = *reinterpret_cast<const f32x4*>(part), w = *reinterpret_cast<const f32x4*>(part + a.dim);
 #pragma unroll
@@ -451,7 +455,7 @@ __global__ __launch_bounds__(NT) void packed_kv_join_kernel(const Args a) {
 }
 
 // How the two kernels are cut. Lengths are on the device, so the rule goes by totals.
-struct Plan { int wk, items, cut_rows, cuts, ktiles; };
+struct Plan { int wk, items, cut_tiles, cuts, ktiles; };
 static Plan plan_of(const dp_packed_attn* d) {
   const int64_t group = d->heads / d->kv_heads, rows = d->tq * group, seqs = std::max(1, d->nseq);
   Plan p{1, 0, 0, 1, 0};
@@ -461,18 +465,22 @@ static Plan plan_of(const dp_packed_attn* d) {
   const int dp = d->dim <= 32 ? 32 : d->dim <= 64 ? 64 : 128, last = d->bias && d->buckets > 2 ? 4096 + 16 : 16;
   if (d->bias && 4 * 32 * p.wk * dp * (d->dtype == DP_F32 ? 4 : 2) / 1024 * 1040 + d->buckets * (NT + (int)group) * 4 + last > 163840) p.wk = 1;
   p.items = (int)(rows / (BM / p.wk) + d->nseq + 1);
-  // a block of keys walks all rows that see them: the longest such walk bounds the time unless it is
-  // cut. About 1024 blocks (causal order leaves half of the cuts empty), at least 512 rows each
+  // The longest walk of a block of keys bounds the time unless it is cut, and a cut costs its start and a part of
+  // dk and dv in f32: about 1536 blocks (in causal order the later keys' walks are short), walks of 256 rows
+  // at least. Causal, dim 128, us with 1024 / 2048 blocks aimed at: 7 k tokens in six sequences, 4 key heads 620 / 555;
+  // 4096 in one, 16 key heads 477 / 537; dim 64 with a bias, 8 key heads 240 / 249 (1536: 572, 495, 249)
+  const int64_t br = d->dtype == DP_F32 || d->dim > 64 ? 32 : 64, walk = (d->tq + br - 1) / br * group;
   const int64_t kblocks = (int64_t)(d->tk / BM + 1) * d->kv_heads;
-  int64_t cuts = std::min<int64_t>(16, (1024 + kblocks - 1) / kblocks * (d->causal ? 2 : 1));
+  int64_t cuts = std::min<int64_t>(16, (1536 + kblocks - 1) / kblocks * (d->causal ? 2 : 1));
   cuts = std::min(cuts, std::max<int64_t>(1, ((int64_t)1 << 30) / std::max<int64_t>(1, (int64_t)d->tk * d->kv_heads * d->dim * 8)));
-  const int64_t per = std::max<int64_t>(512, ((rows + cuts - 1) / cuts + 63) / 64 * 64);
-  cuts = std::min(cuts, (rows + per - 1) / per);
+  const int64_t per = std::max<int64_t>(256 / br, (walk + cuts - 1) / cuts);
+  cuts = std::min(cuts, (walk + per - 1) / per);
   int64_t tiles = d->tk / BM + d->nseq + 1;
   if (cuts > 1) {
     p.cuts = (int)cuts;
-    p.cut_rows = (int)per;
-    tiles = std::min(tiles * cuts, tiles + (d->tk / BM + 1) * (rows / per + 1));
+    p.cut_tiles = (int)per;
+    // a sequence's cuts are at most 1 + its walk / per, and all walks together (walk + a tile a sequence and head) long
+    tiles = std::min(tiles * cuts, tiles + (d->tk / BM + 1) * ((walk + group * seqs) / per + 1));
   }
   p.ktiles = (int)std::min<int64_t>(tiles, INT32_MAX);
   return p;
@@ -497,12 +505,12 @@ int launch_q(const Args& a, hipStream_t s) {
 
 template <typename T, int DP, bool BIAS>
 int launch(const Args& a, int wk, void* dbias, int bias_f32, hipStream_t s) {
-  constexpr int BR = sizeof(T) == 2 ? 64 : 32;
+  constexpr int BR = sizeof(T) == 2 && DP < 128 ? 64 : 32;
   constexpr int W = sizeof(T) == 2 || DP <= 64 ? 4 : 2;
   if (a.tq > 0)
     if (const int rc = wk > 1 ? launch_q<T, DP, W, BIAS>(a, s) : launch_q<T, DP, 1, BIAS>(a, s)) return rc;
   if (a.tk > 0) {
-    const int lds = 4 * Tile<T, DP>::bytes(BR) + 16 * BR * 2 + bias_lds(a);
+    const int lds = 4 * Tile<T, DP>::bytes(BR) + (sizeof(T) == 2 && DP == 128 ? Tile<T, DP>::bytes(BM) : 0) + 16 * BR + bias_lds(a);
     const auto kern = packed_bwd_kv_kernel<T, DP, BR, BIAS>;
     if (const int rc = grow_lds((const void*)kern, lds)) return rc;
     hipLaunchKernelGGL(kern, dim3(a.ktiles * a.hkv), dim3(NT), lds, s, a);
@@ -556,7 +564,7 @@ extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
   a.tiles = p.items;
   a.ktiles = p.ktiles;
   a.cuts = p.cuts;
-  a.cut_rows = p.cut_rows;
+  a.cut_tiles = p.cut_tiles;
   DP_REQUIRE((int64_t)p.ktiles * a.hkv < INT32_MAX, "dp_packed_attn_bwd: too many tiles");
   a.dsum = (float*)d->ws;
   a.dbias_part = a.dsum + (int64_t)d->tq * d->heads;

@@ -58,7 +58,8 @@ __device__ __forceinline__ int splits_of(const Args& a, int lk, int rows) {
 // WK waves of a block share its rows and walk the key tile's subtiles in turn; 4 / WK of them, 32 rows
 // each, lie along the rows.
 template <typename T, int DP, int WK, int BN, bool BIAS>
-__global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packed_fwd_kernel(const Args a, int fill_tail) {
+__global__ __launch_bounds__(NT)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 128 ? 2 : 8))) void packed_fwd_kernel(const Args a, int fill_tail) {
   using TL = Tile<T, DP>;
   constexpr int TB = TL::bytes(BN), NS = BN / 32 / WK, ROWS = BM / WK, OP = DP + 4;
   // waves that lie along the keys load what they read themselves and wait for no other
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) void packe
     return;
   const int q0 = it.start, lq = it.len, k0 = it.start2, lk = it.len2;
   const int cuts = uniform(cuts_of(lq, lk)), ntile = uniform(tiles_of(lq)), cut = uniform(it.sub / ntile);
-  const int off = lk - lq, rows = lq * a.group, row0 = (it.sub - cut * ntile) * ROWS;
+  const int off = lk - lq, rows = lq * a.group, row0 = uniform(it.sub - cut * ntile) * ROWS;
   const int first = row0 + 32 * wr, r = first + (lane & 31);
   const bool ok = r < rows;
   const int rc = min(r, rows - 1), pos = rc / a.group, g = rc - pos * a.group;
