@@ -6,6 +6,7 @@ __graft_entry__.build()).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -83,7 +84,7 @@ class RowCopyDesc(C.Structure):
 
 class PackedAttn(C.Structure):
     """Mirror of dp_packed_attn."""
-    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("out", vp), ("lse", vp),
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("out", vp), ("lse", vp), ("out_lo", vp),
                 ("q_row", i64), ("q_head", i64), ("k_row", i64), ("k_head", i64), ("v_row", i64), ("v_head", i64),
                 ("o_row", i64), ("o_head", i64), ("cu_q", vp), ("cu_k", vp),
                 ("nseq", i32), ("tq", i32), ("tk", i32), ("heads", i32), ("kv_heads", i32), ("dim", i32),
@@ -259,6 +260,15 @@ def verify_source(lib, expected: str | None = None):
     if got != expected:
         raise HipError(f"{LIB_PATH} was built from sources {got}, the shipped sources are {expected}: "
                        f"rebuild it with `python -m detrpose_amd.build`")
+
+
+_here = contextlib.nullcontext()
+
+
+def device_of(t):
+    """A context in which t's GPU is the current one (nothing to do where it is already)."""
+    import torch
+    return _here if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def check(rc: int, what: str = ""):

@@ -85,9 +85,9 @@ def _check(q, k, v, cu_q, cu_k, scale, bias_table, out):
 
 def _ready(t):
     """The tensor, or a contiguous copy where its rows cannot be read in 16-byte pieces."""
-    e = t.element_size()
-    if t.numel() == 0:
+    if t.numel() == 0 or (t.is_contiguous() and t.data_ptr() % 16 == 0):
         return t
+    e = t.element_size()
     ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(s >= 0 and s * e % 16 == 0 for s in t.stride()[:2])
           and t.stride(0) * e < 1 << 24 and t.stride(1) * e * t.shape[1] < 1 << 28)
     return t if ok else t.contiguous()
@@ -97,13 +97,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _desc(q, k, v, out, lse, cu_q, cu_k, causal, scale, table, edges, both, fill_tail):
+def _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, fill_tail):
     a = _lib.PackedAttn()
-    a.q, a.k, a.v, a.out, a.lse = _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse)
-    a.q_row, a.q_head = q.stride(0), q.stride(1)
-    a.k_row, a.k_head = k.stride(0), k.stride(1)
-    a.v_row, a.v_head = v.stride(0), v.stride(1)
-    a.o_row, a.o_head = out.stride(0), out.stride(1)
+    a.q, a.k, a.v, a.out, a.lse, a.out_lo = _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(lo)
+    (a.q_row, a.q_head, _), (a.k_row, a.k_head, _) = q.stride(), k.stride()
+    (a.v_row, a.v_head, _), (a.o_row, a.o_head, _) = v.stride(), out.stride()
     a.cu_q, a.cu_k, a.nseq = _ptr(cu_q), _ptr(cu_k), cu_q.numel() - 1
     a.tq, a.tk, a.heads, a.kv_heads, a.dim = q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
     a.causal, a.fill_tail, a.scale, a.dtype = int(causal), int(fill_tail), scale, _DT[q.dtype]
@@ -114,45 +112,46 @@ def _desc(q, k, v, out, lse, cu_q, cu_k, causal, scale, table, edges, both, fill
 
 
 def _forward(q, k, v, cu_q, cu_k, causal, scale, table, edges, both, out, need_lse):
-    """(out, lse, and the tensors as the kernels read them)."""
+    """(out, lse, what out's rounding left off, and the tensors as the kernels read them)."""
     q, k, v, cu_q, cu_k = _ready(q), _ready(k), _ready(v), cu_q.contiguous(), cu_k.contiguous()
     table = None if table is None else table.contiguous()
     fill = out is None
     if fill:
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lib = _lib.load()
-    with torch.cuda.device(q.device):
+    with _lib.device_of(q):
         lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if need_lse else None
-        a = _desc(q, k, v, out, lse, cu_q, cu_k, causal, scale, table, edges, both, fill)
+        lo = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_lse and q.dtype == torch.bfloat16 else None
+        a = _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, fill)
         nb = int(lib.dp_packed_attn_ws_bytes(C.byref(a), 0))
         ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
         a.ws, a.ws_bytes = _ptr(ws), nb
         s = torch.cuda.current_stream().cuda_stream
         _lib.check(lib.dp_packed_attn_fwd(C.byref(a), C.c_void_p(s)), "dp_packed_attn_fwd")
-    return out, lse, (q, k, v, cu_q, cu_k, table)
+    return out, lse, lo, (q, k, v, cu_q, cu_k, table)
 
 
 class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, causal, scale, edges, both):
         need = any(ctx.needs_input_grad[:4])
-        out, lse, read = _forward(q, k, v, cu_q, cu_k, causal, scale, table, edges, both, None, need)
+        out, lse, lo, read = _forward(q, k, v, cu_q, cu_k, causal, scale, table, edges, both, None, need)
         if need:
-            ctx.save_for_backward(*read, out, lse)
+            ctx.save_for_backward(*read, out, lse, lo)
             ctx.how = (causal, scale, edges, both)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, cu_q, cu_k, table, out, lse = ctx.saved_tensors
+        q, k, v, cu_q, cu_k, table, out, lse, lo = ctx.saved_tensors
         causal, scale, edges, both = ctx.how
         dout = _ready(dout.to(q.dtype))
         lib = _lib.load()
-        with torch.cuda.device(q.device):
+        with _lib.device_of(q):
             dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
             dtable = None if table is None else torch.empty_like(table)
-            a = _desc(q, k, v, out, lse, cu_q, cu_k, causal, scale, table, edges, both, False)
+            a = _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, False)
             a.dout, a.g_row, a.g_head = _ptr(dout), dout.stride(0), dout.stride(1)
             a.dq, a.dk, a.dv, a.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
             nb = int(lib.dp_packed_attn_ws_bytes(C.byref(a), 1))
@@ -204,4 +203,7 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
             raise ValueError(f"packed_attention: out {tuple(out.shape)} {out.dtype} with strides {out.stride()} does not "
                              f"match q {tuple(q.shape)} {q.dtype} in rows of 16-byte pieces")
         return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale, bias_table, edges, both, out, False)[0]
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                         (bias_table is not None and bias_table.requires_grad))):
+        return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale, bias_table, edges, both, None, False)[0]
     return PackedAttentionFunction.apply(q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, bool(causal), scale, edges, both)

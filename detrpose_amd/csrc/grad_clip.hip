@@ -119,7 +119,8 @@ __global__ __launch_bounds__(BT) void grad_scale_kernel(const Table t, const dou
   const double c = (double)max_norm / (len + 1e-6);
   const float coef = c > 1.0 ? 1.f : (float)c;
   if (!out && coef == 1.f) return;
-  for (int tile = blockIdx.x; tile < t.tiles; tile += gridDim.x) {
+  // backwards: what the norm's pass read last is still in the 256 MB behind the L2
+  for (int tile = t.tiles - 1 - blockIdx.x; tile >= 0; tile -= gridDim.x) {
     const int k = slot_of(t, tile);
     const int64_t cnt = t.n[k], n = cnt < 0 ? -cnt : cnt;
     const int64_t a = (int64_t)(tile - t.first[k]) * TILE;
@@ -158,8 +159,6 @@ static int disjoint(void* const* ptr, const int64_t* n, const int32_t* dt, int c
   return 0;
 }
 
-static int grid_of(int tiles) { return std::min(tiles, MAXGRID); }
-
 }  // namespace
 
 extern "C" int64_t dp_grad_clip_ws_bytes(int32_t count) {
@@ -187,33 +186,38 @@ extern "C" int dp_grad_clip(void* const* ptr, const int64_t* n, const int32_t* d
   if (const int rc = disjoint(ptr, n, dtype, count, out, out ? out_n * (out_dtype == DP_BF16 ? 2 : 4) : 0)) return rc;
   hipStream_t s = as_stream(stream);
   double* part = (double*)ws;
-  int parts = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t at = 0;
-    for (int base = 0; base < count; base += SLOTS) {
-      Table t;
-      t.count = std::min(SLOTS, count - base);
-      t.tiles = 0;
-      for (int i = 0; i < t.count; ++i) {
-        const int64_t m = n[base + i];
-        t.p[i] = ptr[base + i];
-        t.n[i] = dtype[base + i] == DP_BF16 ? -m : m;
-        t.at[i] = at;
-        t.first[i] = t.tiles;   // a tensor of no elements has no tile: the search passes over it
-        t.tiles += (int)((m + TILE - 1) / TILE);
-        at += m;
-      }
-      const int grid = grid_of(t.tiles);
-      if (pass == 0) {
-        if (!grid) continue;
-        hipLaunchKernelGGL(grad_sq_kernel, dim3(grid), dim3(BT), 0, s, t, part + parts);
-        parts += grid;
-      } else {
-        if (!grid && base) continue;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(std::max(1, grid)), dim3(BT), 0, s, t, part, parts, max_norm,
-                           base ? nullptr : norm, out, out_dtype == DP_BF16);
-      }
+  const int tables = (count + SLOTS - 1) / SLOTS;
+  auto fill = [&](int base, int64_t at) {
+    Table t;
+    t.count = std::min(SLOTS, count - base);
+    t.tiles = 0;
+    for (int i = 0; i < t.count; ++i) {
+      const int64_t m = n[base + i];
+      t.p[i] = ptr[base + i];
+      t.n[i] = dtype[base + i] == DP_BF16 ? -m : m;
+      t.at[i] = at;
+      t.first[i] = t.tiles;   // a tensor of no elements has no tile: the search passes over it
+      t.tiles += (int)((m + TILE - 1) / TILE);
+      at += m;
     }
+    return t;
+  };
+  int parts = 0;
+  for (int k = 0; k < tables; ++k) {
+    const Table t = fill(k * SLOTS, 0);
+    const int grid = std::min(t.tiles, MAXGRID);
+    if (!grid) continue;
+    hipLaunchKernelGGL(grad_sq_kernel, dim3(grid), dim3(BT), 0, s, t, part + parts);
+    parts += grid;
+  }
+  int64_t at = total;
+  for (int k = tables - 1; k >= 0; --k) {
+    for (int i = k * SLOTS; i < std::min(count, (k + 1) * SLOTS); ++i) at -= n[i];
+    const Table t = fill(k * SLOTS, at);
+    const int grid = std::min(t.tiles, MAXGRID);
+    if (grid || k == 0)
+      hipLaunchKernelGGL(grad_scale_kernel, dim3(std::max(1, grid)), dim3(BT), 0, s, t, part, parts, max_norm,
+                         k ? nullptr : norm, out, out_dtype == DP_BF16);
   }
   return dp_check_launch("dp_grad_clip");
 }

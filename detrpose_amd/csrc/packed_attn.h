@@ -42,6 +42,7 @@ struct Args {
   const void *q, *k, *v;
   void* out;
   float* lse;
+  bf16_t* out_lo;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   const int32_t *cu_q, *cu_k;
   int nseq, tq, tk, hkv, group, dim, causal, tiles;
@@ -319,6 +320,24 @@ __device__ __forceinline__ float half_max(float x) {
 __device__ __forceinline__ void tile_barrier() {
   dpconv::wait_vmcnt<0>();
   __syncthreads();
+}
+
+// four results of a row: rounded, and in bf16, where the backward wants it, what the rounding left off
+template <typename T>
+__device__ __forceinline__ void put4(T* out, bf16_t* lo, const f32x4& x) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(x[e]);
+  *reinterpret_cast<T4*>(out) = w;
+  if constexpr (sizeof(T) == 2) {
+    if (lo) {
+      bf16x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (bf16_t)(x[e] - (float)w[e]);
+      *reinterpret_cast<bf16x4*>(lo) = r;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- which sequence a block works on

@@ -78,6 +78,18 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
 #pragma unroll
       for (int e = 0; e < TL::VN; ++e) D = fmaf(to_f32(x[e]), to_f32(y[e]), D);
     }
+    if constexpr (sizeof(T) == 2) {
+      if (a.out_lo) {
+        load_frags<T, DP>(a.out_lo + at * a.dim, ok, a.dim, h, of);
+#pragma unroll
+        for (int s = 0; s < TL::KS; ++s) {
+          const T* x = reinterpret_cast<const T*>(&of[s]);
+          const T* y = reinterpret_cast<const T*>(&gf[s]);
+#pragma unroll
+          for (int e = 0; e < TL::VN; ++e) D = fmaf(to_f32(x[e]), to_f32(y[e]), D);
+        }
+      }
+    }
     D = half_sum(D);
   }
   if (ok && h == 0 && wk == 0) a.dsum[at] = D;

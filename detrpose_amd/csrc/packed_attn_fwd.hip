@@ -46,8 +46,14 @@ __device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos,
   sum = wave_sum(sum);
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* o = (T*)a.out + (int64_t)(q0 + pos) * a.o_row + head * a.o_head;
-  if (lane < a.dim) o[lane] = from_f32<T>(o0 * inv);
-  if (lane + 64 < a.dim) o[lane + 64] = from_f32<T>(o1 * inv);
+  bf16_t* lo = a.out_lo ? a.out_lo + ((int64_t)(q0 + pos) * a.hkv * a.group + head) * a.dim : nullptr;
+#pragma unroll
+  for (int d = lane; d < 128; d += 64)
+    if (d < a.dim) {
+      const float x = (d == lane ? o0 : o1) * inv;
+      o[d] = from_f32<T>(x);
+      if (lo) lo[d] = (bf16_t)(x - to_f32(o[d]));
+    }
 }
 
 // chunks that a sequence's keys are cut into, for a tile of `rows` rows
@@ -203,11 +209,8 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
     if (cuts > 1) {
       *reinterpret_cast<f32x4*>(a.part + ((int64_t)cut * a.tq * heads + at) * a.dim + d) = x;
     } else {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      T4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = from_f32<T>(x[i]);
-      *reinterpret_cast<T4*>((T*)a.out + (int64_t)(q0 + p) * a.o_row + (kvh * a.group + hd) * a.o_head + d) = w;
+      put4<T>((T*)a.out + (int64_t)(q0 + p) * a.o_row + (kvh * a.group + hd) * a.o_head + d,
+              a.out_lo ? a.out_lo + at * a.dim + d : nullptr, x);
     }
   };
   auto put_lse = [&](int64_t at, float mm, float ll) {
@@ -367,12 +370,9 @@ __global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
       bad |= sum[e] != sum[e];
     }
     if (d < a.dim) {
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      T4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = from_f32<T>(sum[e]);
       const int64_t row = at / heads;
-      *reinterpret_cast<T4*>((T*)a.out + row * a.o_row + (at - row * heads) * a.o_head + d) = w;
+      put4<T>((T*)a.out + row * a.o_row + (at - row * heads) * a.o_head + d,
+              a.out_lo ? a.out_lo + at * a.dim + d : nullptr, sum);
     }
     if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : (BIAS ? ref + __logf(tot) : ref + __log2f(tot));
   }
@@ -422,15 +422,12 @@ __global__ __launch_bounds__(NT) void packed_join_row_kernel(const Args a) {
     for (int k = 1; k < GROUPS; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += sm[k * TPR + threadIdx.x][e];
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T4 w;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       sum[e] *= inv;
       bad |= sum[e] != sum[e];
-      w[e] = from_f32<T>(sum[e]);
     }
-    *reinterpret_cast<T4*>((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d) = w;
+    put4<T>((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, a.out_lo ? a.out_lo + at * a.dim + d : nullptr, sum);
     if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : ref + (BIAS ? __logf(tot) : __log2f(tot));
   }
   if (threadIdx.x < 64 && __ballot(bad)) redo_row<T>(a, row, head);
@@ -522,6 +519,8 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
   DP_REQUIRE((d->cu_q && d->cu_k) || d->nseq == 0, "%s: no sequence offsets", what);
   DP_REQUIRE((d->q && d->out) || d->tq == 0, "%s: no queries or output", what);
   DP_REQUIRE((d->k && d->v) || d->tk == 0, "%s: no keys or values", what);
+  DP_REQUIRE(!d->out_lo || (d->dtype == DP_BF16 && d->lse && (uintptr_t)d->out_lo % 16 == 0),
+             "%s: out_lo goes with bf16 and lse, 16-byte aligned", what);
   const int e = d->dtype == DP_BF16 ? 2 : 4;
   struct { const char* name; const void* p; int64_t row, head; } t[] = {
       {"q", d->q, d->q_row, d->q_head}, {"k", d->k, d->k_row, d->k_head}, {"v", d->v, d->v_row, d->v_head},
@@ -535,7 +534,7 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
                "%s: strides of %s too large", what, t[i].name);
   }
   *a = dppa::Args{};
-  a->q = d->q; a->k = d->k; a->v = d->v; a->out = d->out; a->lse = d->lse;
+  a->q = d->q; a->k = d->k; a->v = d->v; a->out = d->out; a->lse = d->lse; a->out_lo = (bf16_t*)d->out_lo;
   a->q_row = d->q_row; a->q_head = d->q_head; a->k_row = d->k_row; a->k_head = d->k_head;
   a->v_row = d->v_row; a->v_head = d->v_head; a->o_row = d->o_row; a->o_head = d->o_head;
   a->cu_q = d->cu_q; a->cu_k = d->cu_k; a->nseq = d->nseq; a->tq = d->tq; a->tk = d->tk;

@@ -6,7 +6,7 @@
 //
 // Sums, rstd and dw are f32 throughout. Bound by HBM: the forward reads x, res and writes r, y once
 // each, the backward reads r, dy, dres and writes dr; a row stays in registers between the passes.
-// TPR threads own a row (64: one wave, no barrier; 256: one block), each V vectors of 16 bytes at
+// TPR threads own a row (up to 64: lanes of one wave, no barrier; from 256: one block), each V vectors of 16 bytes at
 // vector index t + TPR i, so every access of a wave is 1 KB contiguous. Rows need only their
 // element's alignment (the loads are declared so and stay 16 bytes wide); the last, partial vector
 // of a row whose length is no multiple of the vector is read and written element by element.
@@ -15,8 +15,9 @@
 
 namespace {
 
-constexpr int BT = 256;   // threads of a block
-constexpr int MAXV = 8;   // vectors a thread: rows of up to 256 * 8 vectors
+constexpr int BT = 256;         // threads of a block whose rows take no more
+constexpr int MOST = 2 * 1024;  // vectors of a row at most
+template <int TPR> constexpr int threads() { return TPR > BT ? TPR : BT; }
 
 template <typename T> constexpr int vn() { return 16 / (int)sizeof(T); }
 
@@ -25,19 +26,33 @@ struct __attribute__((packed, aligned(sizeof(T)))) Raw16 {
   T e[16 / sizeof(T)];
 };
 
-// vector i of a row of c elements as f32 (zero past the end)
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+// vector i of a row of c elements, as it lies there (zero past the end), and its elements as f32
 template <typename T>
-__device__ __forceinline__ void row_load(const T* __restrict__ p, int i, int c, float (&v)[vn<T>()]) {
+__device__ __forceinline__ u32x4_t raw_load(const T* __restrict__ p, int i, int c) {
   constexpr int N = vn<T>();
   const int at = i * N;
-  if (at + N <= c) {
-    const Raw16<T> u = *reinterpret_cast<const Raw16<T>*>(p + at);
+  if (at + N <= c) return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const Raw16<T>*>(p + at));
+  u32x4_t u = {0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = to_f32(u.e[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = at + e < c ? to_f32(p[at + e]) : 0.f;
+  for (int e = 0; e < N; ++e) {
+    if (at + e >= c) continue;
+    if constexpr (sizeof(T) == 2) u[e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[at + e]) << (16 * (e & 1));
+    else u[e] = __builtin_bit_cast(uint32_t, p[at + e]);
   }
+  return u;
+}
+template <typename T>
+__device__ __forceinline__ float element(const u32x4_t& u, int e) {
+  if constexpr (sizeof(T) == 2) return __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+  else return __uint_as_float(u[e]);
+}
+template <typename T>
+__device__ __forceinline__ void row_load(const T* __restrict__ p, int i, int c, float (&v)[vn<T>()]) {
+  const u32x4_t u = raw_load<T>(p, i, c);
+#pragma unroll
+  for (int e = 0; e < vn<T>(); ++e) v[e] = element<T>(u, e);
 }
 
 template <typename T, int N>
@@ -83,7 +98,11 @@ __device__ __forceinline__ void weight_load(const W* __restrict__ w, int i, int 
 // sum (or maximum) over the TPR threads of a row; red: one slot per wave, one call's own
 template <int TPR, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* red) {
-  v = MAX ? wave_max(v) : wave_sum(v);
+#pragma unroll
+  for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) {
+    const float u = __shfl_xor(v, o, 64);
+    v = MAX ? fmaxf(v, u) : v + u;
+  }
   if constexpr (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) red[wave] = v;
@@ -104,16 +123,16 @@ __device__ __forceinline__ unsigned pack_e4m3(float a, float b, float c, float d
 }
 
 template <typename T, typename W, int TPR, int V, bool E4M3>
-__global__ __launch_bounds__(BT) void rms_fwd_kernel(void* __restrict__ yv, float* __restrict__ scale,
+__global__ __launch_bounds__(threads<TPR>()) void rms_fwd_kernel(void* __restrict__ yv, float* __restrict__ scale,
                                                      T* __restrict__ r, float* __restrict__ rstd_out,
                                                      const T* __restrict__ x, int64_t ld_x,
                                                      const T* __restrict__ res, int64_t ld_res,
                                                      const W* __restrict__ w, float eps, int rows, int c) {
   constexpr int N = vn<T>();
-  __shared__ float red[2][BT / 64];
-  const int row = blockIdx.x * (BT / TPR) + threadIdx.x / TPR;
+  __shared__ float red[2][threads<TPR>() / 64];
+  const int row = blockIdx.x * (threads<TPR>() / TPR) + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
-  if (row >= rows) return;   // TPR = 256: one row a block, uniform; TPR = 64: no barrier below
+  if (row >= rows) return;   // TPR >= 256: one row a block, uniform; else no barrier below
   const T* xp = x + (int64_t)row * ld_x;
   const T* rp = res ? res + (int64_t)row * ld_res : nullptr;
   T* sp = r ? r + (int64_t)row * c : nullptr;
@@ -179,18 +198,20 @@ __global__ __launch_bounds__(BT) void rms_fwd_kernel(void* __restrict__ yv, floa
   }
 }
 
-// One block (or one wave of it) walks rows blockIdx, + grid, ...: its dw stays in registers and is
-// written once, part[block (x wave)][c]; rms_dw_kernel adds the parts in a fixed order.
+// A block walks rows blockIdx, + grid, ... (as many at once as it holds), the next row's loads in flight
+// while this one is reduced; its dw stays in registers, is added over the block's rows at once, and is written
+// once, part[block][c]; rms_dw_kernel adds the parts in a fixed order.
 template <typename T, typename W, int TPR, int V>
-__global__ __launch_bounds__(BT) void rms_bwd_kernel(T* __restrict__ dx, float* __restrict__ part,
+__global__ __launch_bounds__(threads<TPR>()) void rms_bwd_kernel(T* __restrict__ dx, float* __restrict__ part,
                                                      const T* __restrict__ r, int64_t ld_r,
                                                      const float* __restrict__ rstd, const T* __restrict__ dy,
                                                      int64_t ld_dy, const T* __restrict__ dres, int64_t ld_dres,
                                                      const W* __restrict__ w, int rows, int c) {
-  constexpr int N = vn<T>(), RPB = BT / TPR;
-  __shared__ float red[2][BT / 64];
+  constexpr int N = vn<T>(), RPB = threads<TPR>() / TPR;
+  __shared__ float red[2][threads<TPR>() / 64];
+  __shared__ float dws[RPB > 1 ? BT * V * N : 1];
   const int sub = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  const int slot = blockIdx.x * RPB + sub;
+  const int64_t step = (int64_t)gridDim.x * RPB;
   float dw[V][N], wv[V][N];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -198,76 +219,114 @@ __global__ __launch_bounds__(BT) void rms_bwd_kernel(T* __restrict__ dx, float* 
 #pragma unroll
     for (int e = 0; e < N; ++e) dw[i][e] = 0.f;
   }
-  int flip = 0;
-  for (int row = slot; row < rows; row += gridDim.x * RPB) {
-    float a[V][N], g[V][N];
+  u32x4_t rr[V], rg[V], rd[V];
+  float rs = 0.f;
+  auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+    if (row >= rows) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      row_load<T>(r + (int64_t)row * ld_r, t + TPR * i, c, a[i]);
-      row_load<T>(dy + (int64_t)row * ld_dy, t + TPR * i, c, g[i]);
+      rr[i] = raw_load<T>(r + row * ld_r, t + TPR * i, c);
+      rg[i] = raw_load<T>(dy + row * ld_dy, t + TPR * i, c);
+      if (dres) rd[i] = raw_load<T>(dres + row * ld_dres, t + TPR * i, c);
     }
-    const float rs = rstd[row];
-    float dot = 0.f;
+    rs = rstd[row];
+  };
+  int64_t row = (int64_t)blockIdx.x * RPB + sub;
+  fetch(row);
+  int flip = 0;
+  for (; row < rows; row += step) {
+    float a[V][N], g[V][N];
+    u32x4_t b[V];
+    const float s = rs;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+    for (int i = 0; i < V; ++i) {
+      b[i] = rd[i];
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        a[i][e] *= rs;
+        a[i][e] = element<T>(rr[i], e) * s;
+        g[i][e] = element<T>(rg[i], e);
+      }
+    }
+    fetch(row + step);
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
         dw[i][e] = fmaf(g[i][e], a[i][e], dw[i][e]);
         g[i][e] *= wv[i][e];
         dot = fmaf(g[i][e], a[i][e], dot);
       }
+    }
     dot = row_reduce<TPR, false>(dot, red[flip]) / (float)c;
     flip ^= 1;   // the other slots next: a wave may still read these
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      float b[N];
-      if (dres) row_load<T>(dres + (int64_t)row * ld_dres, t + TPR * i, c, b);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float d = rs * (g[i][e] - a[i][e] * dot);
-        g[i][e] = dres ? d + b[e] : d;
+        const float d = s * (g[i][e] - a[i][e] * dot);
+        g[i][e] = dres ? d + element<T>(b[i], e) : d;
       }
-      row_store<T, N>(dx + (int64_t)row * c, t + TPR * i, c, g[i]);
+      row_store<T, N>(dx + row * c, t + TPR * i, c, g[i]);
     }
   }
+  float* out = part + (int64_t)blockIdx.x * c;
+  if constexpr (RPB == 1) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) row_store<float, N>(part + (int64_t)slot * c, t + TPR * i, c, dw[i]);
+    for (int i = 0; i < V; ++i) row_store<float, N>(out, t + TPR * i, c, dw[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) dws[sub * (TPR * V * N) + (t + TPR * i) * N + e] = dw[i][e];
+    __syncthreads();
+    for (int j = threadIdx.x; j < c; j += BT) {
+      float x = dws[j];
+#pragma unroll
+      for (int k = 1; k < RPB; ++k) x += dws[k * (TPR * V * N) + j];
+      out[j] = x;
+    }
+  }
 }
 
-// dw[j] = sum over parts, in order: 64 columns x 4 groups of parts a block
+// dw[j] = sum over parts, in order: 16 columns x 16 groups of parts a block
 template <typename W>
 __global__ __launch_bounds__(BT) void rms_dw_kernel(W* __restrict__ dw, const float* __restrict__ part, int parts,
                                                     int c) {
   __shared__ float sm[BT];
-  const int j = blockIdx.x * 64 + (threadIdx.x & 63), grp = threadIdx.x >> 6;
+  const int col = threadIdx.x & 15, j = blockIdx.x * 16 + col, grp = threadIdx.x >> 4;
   float s = 0.f;
   if (j < c) {
-    const int n = (parts + 3) / 4, p0 = grp * n, p1 = min(parts, p0 + n);
+    const int n = (parts + 15) / 16, p0 = grp * n, p1 = min(parts, p0 + n);
 #pragma unroll 8
     for (int p = p0; p < p1; ++p) s += part[(int64_t)p * c + j];
   }
   sm[threadIdx.x] = s;
   __syncthreads();
   if (grp == 0 && j < c) {
-    s = (sm[threadIdx.x] + sm[threadIdx.x + 64]) + (sm[threadIdx.x + 128] + sm[threadIdx.x + 192]);
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sm[16 * k + col];
     dw[j] = from_f32<W>(s);
   }
 }
 
-// threads a row and vectors a thread for rows of c elements: one wave while a row is at most 4
-// vectors a lane, else a block
+// Threads a row and vectors a thread (two at most: the backward keeps a row, the next one, the weights and dw) for
+// rows of c elements: as few lanes as hold a row of up to 64 vectors, a wave for up to 128, else a block
 struct Shape { int tpr, v; };
 static Shape shape_of(int c, int n) {
   const int vec = (c + n - 1) / n;
-  Shape s{vec <= 4 * 64 ? 64 : 256, 1};
-  while (s.v * s.tpr < vec) s.v *= 2;
+  Shape s{8, 1};
+  while (s.tpr < vec && s.tpr < 64) s.tpr *= 2;
+  if (vec > 128) s.tpr = vec > 1024 ? 1024 : vec > 512 ? 512 : 256;
+  if (s.tpr < vec) s.v = 2;
+  if (s.tpr > 256) s.v = 2;
   return s;
 }
 
+// blocks of the backward: up to 4 a CU
 static int bwd_parts(int rows, const Shape& s) {
-  const int rpb = BT / s.tpr;
-  return std::min(512, (rows + rpb - 1) / rpb) * rpb;
+  const int rpb = std::max(1, BT / s.tpr);
+  return std::min(1024, (rows + rpb - 1) / rpb);
 }
 
 struct FwdArgs {
@@ -277,8 +336,8 @@ struct FwdArgs {
 
 template <typename T, typename W, int TPR, int V, bool E4M3>
 void fwd_launch(const FwdArgs& a) {
-  const int rpb = BT / TPR;
-  hipLaunchKernelGGL((rms_fwd_kernel<T, W, TPR, V, E4M3>), dim3((a.rows + rpb - 1) / rpb), dim3(BT), 0, a.s, a.y,
+  const int rpb = threads<TPR>() / TPR;
+  hipLaunchKernelGGL((rms_fwd_kernel<T, W, TPR, V, E4M3>), dim3((a.rows + rpb - 1) / rpb), dim3(threads<TPR>()), 0, a.s, a.y,
                      a.scale, (T*)a.r, a.rstd, (const T*)a.x, a.ld_x, (const T*)a.res, a.ld_res, (const W*)a.w, a.eps,
                      a.rows, a.c);
 }
@@ -288,8 +347,9 @@ int fwd_shape(const FwdArgs& a) {
   const Shape s = shape_of(a.c, vn<T>());
 #define DP_RMS_CASE(TPR_, V_) \
   if (s.tpr == TPR_ && s.v == V_) { fwd_launch<T, W, TPR_, V_, E4M3>(a); return dp_check_launch("dp_rms_norm"); }
-  DP_RMS_CASE(64, 1) DP_RMS_CASE(64, 2) DP_RMS_CASE(64, 4)
-  DP_RMS_CASE(256, 2) DP_RMS_CASE(256, 4) DP_RMS_CASE(256, 8)
+  DP_RMS_CASE(8, 1) DP_RMS_CASE(16, 1) DP_RMS_CASE(32, 1)
+  DP_RMS_CASE(64, 1) DP_RMS_CASE(64, 2) DP_RMS_CASE(256, 1)
+  DP_RMS_CASE(256, 2) DP_RMS_CASE(512, 2) DP_RMS_CASE(1024, 2)
 #undef DP_RMS_CASE
   dp_set_error("dp_rms_norm: rows of %d elements are too long", a.c);
   return DP_EINVAL;
@@ -304,7 +364,7 @@ int fwd_types(const FwdArgs& a, int dtype, int w_dtype) {
 static int check_types(int dtype, int w_dtype, int c) {
   DP_REQUIRE(dtype == DP_F32 || dtype == DP_BF16, "dp_rms_norm: dtype %d", dtype);
   DP_REQUIRE(w_dtype == DP_F32 || w_dtype == dtype, "dp_rms_norm: weights are f32 or of the activations' type");
-  const int most = BT * MAXV * (dtype == DP_F32 ? 4 : 8);
+  const int most = MOST * (dtype == DP_F32 ? 4 : 8);
   DP_REQUIRE(c > 0 && c <= most, "dp_rms_norm: rows of %d elements (1 to %d)", c, most);
   return 0;
 }
@@ -313,15 +373,16 @@ template <typename T, typename W>
 int bwd_shape(void* dx, float* part, const void* r, int64_t ld_r, const float* rstd, const void* dy, int64_t ld_dy,
               const void* dres, int64_t ld_dres, const void* w, void* dw, int rows, int c, hipStream_t st) {
   const Shape s = shape_of(c, vn<T>());
-  const int parts = bwd_parts(rows, s), grid = parts / (BT / s.tpr);
+  const int parts = bwd_parts(rows, s);
 #define DP_RMS_CASE(TPR_, V_)                                                                                        \
   if (s.tpr == TPR_ && s.v == V_)                                                                                    \
-    hipLaunchKernelGGL((rms_bwd_kernel<T, W, TPR_, V_>), dim3(grid), dim3(BT), 0, st, (T*)dx, part, (const T*)r, ld_r, \
+    hipLaunchKernelGGL((rms_bwd_kernel<T, W, TPR_, V_>), dim3(parts), dim3(threads<TPR_>()), 0, st, (T*)dx, part, (const T*)r, ld_r, \
                        rstd, (const T*)dy, ld_dy, (const T*)dres, ld_dres, (const W*)w, rows, c);
-  DP_RMS_CASE(64, 1) DP_RMS_CASE(64, 2) DP_RMS_CASE(64, 4)
-  DP_RMS_CASE(256, 2) DP_RMS_CASE(256, 4) DP_RMS_CASE(256, 8)
+  DP_RMS_CASE(8, 1) DP_RMS_CASE(16, 1) DP_RMS_CASE(32, 1)
+  DP_RMS_CASE(64, 1) DP_RMS_CASE(64, 2) DP_RMS_CASE(256, 1)
+  DP_RMS_CASE(256, 2) DP_RMS_CASE(512, 2) DP_RMS_CASE(1024, 2)
 #undef DP_RMS_CASE
-  hipLaunchKernelGGL((rms_dw_kernel<W>), dim3((c + 63) / 64), dim3(BT), 0, st, (W*)dw, part, parts, c);
+  hipLaunchKernelGGL((rms_dw_kernel<W>), dim3((c + 15) / 16), dim3(BT), 0, st, (W*)dw, part, parts, c);
   return dp_check_launch("dp_rms_norm_bwd");
 }
 
@@ -350,7 +411,7 @@ extern "C" int dp_rms_norm_e4m3(void* y, float* scale, void* r, const void* x, i
 }
 
 extern "C" int64_t dp_rms_norm_bwd_ws_floats(int32_t rows, int32_t c, int32_t dtype) {
-  if (rows <= 0 || c <= 0 || c > BT * MAXV * (dtype == DP_F32 ? 4 : 8)) return 0;
+  if (rows <= 0 || c <= 0 || c > MOST * (dtype == DP_F32 ? 4 : 8)) return 0;
   return (int64_t)bwd_parts(rows, shape_of(c, dtype == DP_F32 ? 4 : 8)) * c;
 }
 

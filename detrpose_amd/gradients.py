@@ -9,6 +9,7 @@ There is no CPU path: the HIP library must load (see _lib.load()).
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 
 import torch
@@ -55,9 +56,9 @@ def clip_grad_norm_(parameters, max_norm, out=None):
     kinds = {g.dtype for g in grads}
     if kinds - _DT.keys():
         raise TypeError(f"clip_grad_norm_: gradient dtypes {sorted(map(str, kinds))} (f32 / bf16)")
-    if any(g.layout != torch.strided for g in grads):
-        raise TypeError("clip_grad_norm_: sparse gradients")
-    if device.type != "cuda" or len(set(map(torch.Tensor.get_device, grads))) != 1:
+    if len(set(map(torch.Tensor.get_device, grads))) != 1 or device.type != "cuda" or grads[0].layout != torch.strided:
+        if any(g.layout != torch.strided for g in grads):
+            raise TypeError("clip_grad_norm_: sparse gradients")
         raise RuntimeError("clip_grad_norm_: gradients must be on one GPU (no CPU path)")
     sizes = list(map(torch.Tensor.numel, grads))
     if out is not None:
@@ -69,26 +70,29 @@ def clip_grad_norm_(parameters, max_norm, out=None):
             raise ValueError(f"clip_grad_norm_: out {tuple(out.shape)} is not a contiguous row of {sum(sizes)} elements")
         if out.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("clip_grad_norm_: out requires a gradient")
-    for i, ok in enumerate(map(torch.Tensor.is_contiguous, grads)):
-        if ok:
-            continue
+    try:
+        plain = list(map(torch.Tensor.is_contiguous, grads))
+    except RuntimeError:   # a sparse tensor has no strides
+        raise TypeError("clip_grad_norm_: sparse gradients") from None
+    for i in (i for i, ok in enumerate(plain) if not ok) if not all(plain) else ():
         if out is not None:
             grads[i] = grads[i].contiguous()   # out takes the elements in their logical order
         elif not _dense(grads[i]):
             raise ValueError(f"clip_grad_norm_: gradient {i} {tuple(grads[i].shape)} with strides {grads[i].stride()} "
                              "does not fill one span of memory: clip a contiguous copy")
     n = len(grads)
-    ptrs = (C.c_void_p * n)(*map(torch.Tensor.data_ptr, grads))
-    nums = (C.c_int64 * n)(*sizes)
-    dts = (C.c_int32 * n)(*[_DT[g.dtype] for g in grads]) if len(kinds) > 1 else (C.c_int32 * n)(*[_DT[grads[0].dtype]] * n)
+    ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+    nums = array.array("q", sizes)
+    dts = array.array("i", [_DT[g.dtype] for g in grads] if len(kinds) > 1 else [_DT[grads[0].dtype]]) * (n if len(kinds) == 1 else 1)
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _lib.device_of(grads[0]):
         norm = torch.empty((), device=device, dtype=torch.float32)
         nb = int(lib.dp_grad_clip_ws_bytes(n))
         ws = torch.empty(nb, device=device, dtype=torch.uint8)
         s = torch.cuda.current_stream().cuda_stream
-        _lib.check(lib.dp_grad_clip(ptrs, nums, dts, n, max_norm, norm.data_ptr(),
-                                    None if out is None else out.data_ptr(), 0 if out is None else out.numel(),
+        _lib.check(lib.dp_grad_clip(ptrs.buffer_info()[0], nums.buffer_info()[0], dts.buffer_info()[0], n, max_norm,
+                                    norm.data_ptr(), None if out is None else out.data_ptr(),
+                                    0 if out is None else out.numel(),
                                     _lib.DP_F32 if out is None else _DT[out.dtype], ws.data_ptr(), nb,
                                     C.c_void_p(s)), "dp_grad_clip")
     return norm

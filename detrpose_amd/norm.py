@@ -69,7 +69,7 @@ class RMSNormFunction(torch.autograd.Function):
         need = any(ctx.needs_input_grad[:3])
         rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if need else None
         if rows:
-            with torch.cuda.device(x.device):
+            with _lib.device_of(x):
                 s = torch.cuda.current_stream().cuda_stream
                 _lib.check(_lib.load().dp_rms_norm(y.data_ptr(), _ptr(r), _ptr(rstd), xm.data_ptr(), ld_x, _ptr(rm),
                                                    ld_r, w.data_ptr(), _DT[w.dtype], eps, rows, c, _DT[x.dtype],
@@ -97,7 +97,7 @@ class RMSNormFunction(torch.autograd.Function):
         dym, ld_dy = _rows(dy.to(r.dtype), c)
         drm, ld_dr = (None, 0) if dres is None else _rows(dres.to(r.dtype), c)
         lib = _lib.load()
-        with torch.cuda.device(r.device):
+        with _lib.device_of(r):
             n = int(lib.dp_rms_norm_bwd_ws_floats(rows, c, _DT[r.dtype]))
             ws = torch.empty(n, device=r.device, dtype=torch.float32)
             s = torch.cuda.current_stream().cuda_stream
@@ -135,7 +135,7 @@ def rms_norm_e4m3(x, weight, residual=None, eps=1e-6):
         rm, ld_r = _rows(residual, c)
         r = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     if rows:
-        with torch.cuda.device(x.device):
+        with _lib.device_of(x):
             s = torch.cuda.current_stream().cuda_stream
             _lib.check(_lib.load().dp_rms_norm_e4m3(y.data_ptr(), scale.data_ptr(), _ptr(r), xm.data_ptr(), ld_x,
                                                     _ptr(rm), ld_r, w.data_ptr(), _DT[w.dtype], eps, rows, c,

@@ -745,6 +745,8 @@ int dp_maxpool2x2_pad_rb_bwd(const void* x, int64_t x_bstride, int32_t x_pstride
  *  q, out [tq][heads][dim], k, v [tk][kv_heads][dim] of dtype, element strides *_row / *_head, dim
  *  contiguous, every row 16-byte aligned; dim a multiple of 8 up to 128.
  *  lse: f32 [tq][heads] (the log of the softmax's denominator, in the backward's units), or NULL.
+ *  out_lo: NULL, or bf16 [tq][heads][dim] contiguous (dtype bf16 with lse): what out's rounding left off,
+ *  out + out_lo being out to 16 bits. The backward's D = sum dout out takes it in when it is given.
  *  bias: NULL or a learned table [buckets][heads] (f32, or dtype): the bias of pair (i, j) is
  *  bias[bucket(j - position)][h]. n = |j - position| (one direction: max(position - j, 0)) falls into
  *  the bucket numbered by how many of edge[0 .. nb - 2] are <= n, nb = buckets (both directions: half of
@@ -755,6 +757,7 @@ typedef struct dp_packed_attn {
   const void *q, *k, *v;
   void* out;
   float* lse;
+  void* out_lo;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   const int32_t *cu_q, *cu_k;
   int32_t nseq, tq, tk, heads, kv_heads, dim, causal, fill_tail;
