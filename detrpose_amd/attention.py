@@ -32,7 +32,7 @@ def bucket_edges(num_buckets, max_distance, bidirectional):
     nb = num_buckets // 2 if bidirectional else num_buckets
     e = nb // 2
     if not (2 <= num_buckets <= 64 and nb >= 2):
-        raise ValueError(f"packed_attention: {num_buckets} buckets (2 to 64 a direction's, at least 2 each)")
+        raise ValueError(f"packed_attention: {num_buckets} buckets (2 to 64, at least 2 a direction)")
     if not e < max_distance <= 4096:
         raise ValueError(f"packed_attention: max_distance {max_distance} ({e + 1} to 4096 with {num_buckets} buckets)")
     k = nb - e
@@ -87,10 +87,38 @@ def _ready(t):
     """The tensor, or a contiguous copy where its rows cannot be read in 16-byte pieces."""
     if t.numel() == 0 or (t.is_contiguous() and t.data_ptr() % 16 == 0):
         return t
-    e = t.element_size()
-    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(s >= 0 and s * e % 16 == 0 for s in t.stride()[:2])
-          and t.stride(0) * e < 1 << 24 and t.stride(1) * e * t.shape[1] < 1 << 28)
+    e, (row, head) = t.element_size(), _strides(t)
+    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and row * e % 16 == 0 and head * e % 16 == 0
+          and row * e < 1 << 24 and head * e * t.shape[1] < 1 << 28)
     return t if ok else t.contiguous()
+
+
+def _strides(t):
+    """(row, head) in elements; a tensor may have any stride along a dimension of one."""
+    return (t.stride(0) if t.shape[0] > 1 else t.shape[2]), (t.stride(1) if t.shape[1] > 1 else t.shape[2])
+
+
+def _span(t):
+    """First byte and the one behind the last of a tensor that is not empty."""
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _check_out(q, k, v, cu_q, cu_k, table, out):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table, out)):
+        raise RuntimeError("packed_attention: out= has no gradient (call it under torch.no_grad())")
+    if out.shape != q.shape or out.dtype != q.dtype or (out.numel() and _ready(out) is not out):
+        raise ValueError(f"packed_attention: out {tuple(out.shape)} {out.dtype} with strides {out.stride()} does not "
+                         f"match q {tuple(q.shape)} {q.dtype} in rows of 16-byte pieces")
+    if not out.numel():
+        return
+    (row, head), (n, h, d) = _strides(out), out.shape
+    if not ((head >= d or h == 1) and (row >= (h - 1) * head + d or n == 1)
+            or (row >= d or n == 1) and (head >= (n - 1) * row + d or h == 1)):
+        raise ValueError(f"packed_attention: rows of out {tuple(out.shape)} with strides {out.stride()} overlap")
+    a, b = _span(out)
+    for name, t in (("q", q), ("k", k), ("v", v), ("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k), ("bias_table", table)):
+        if t is not None and t.numel() and a < _span(t)[1] and _span(t)[0] < b:
+            raise ValueError(f"packed_attention: out lies across {name}, which is read while out is written")
 
 
 def _ptr(t):
@@ -100,8 +128,8 @@ def _ptr(t):
 def _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, fill_tail):
     a = _lib.PackedAttn()
     a.q, a.k, a.v, a.out, a.lse, a.out_lo = _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(lo)
-    (a.q_row, a.q_head, _), (a.k_row, a.k_head, _) = q.stride(), k.stride()
-    (a.v_row, a.v_head, _), (a.o_row, a.o_head, _) = v.stride(), out.stride()
+    (a.q_row, a.q_head), (a.k_row, a.k_head) = _strides(q), _strides(k)
+    (a.v_row, a.v_head), (a.o_row, a.o_head) = _strides(v), _strides(out)
     a.cu_q, a.cu_k, a.nseq = _ptr(cu_q), _ptr(cu_k), cu_q.numel() - 1
     a.tq, a.tk, a.heads, a.kv_heads, a.dim = q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2]
     a.causal, a.fill_tail, a.scale, a.dtype = int(causal), int(fill_tail), scale, _DT[q.dtype]
@@ -152,7 +180,7 @@ class PackedAttentionFunction(torch.autograd.Function):
             dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
             dtable = None if table is None else torch.empty_like(table)
             a = _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, False)
-            a.dout, a.g_row, a.g_head = _ptr(dout), dout.stride(0), dout.stride(1)
+            a.dout, (a.g_row, a.g_head) = _ptr(dout), _strides(dout)
             a.dq, a.dk, a.dv, a.dbias = _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
             nb = int(lib.dp_packed_attn_ws_bytes(C.byref(a), 1))
             ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
@@ -185,7 +213,7 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     k, v and bias_table, with equal bits for equal inputs; gradients of rows behind the last sequence are
     zeros. Scores and sums are f32; in bf16 the weights (and their gradients) are rounded to bf16 for the
     products with v, q and k. out: the result is written here instead, rows behind the last sequence are left
-    as they are; without gradients only.
+    as they are; without gradients only, and in memory apart from what is read.
     Values that causal order hides from a query do not reach its output, be they inf or NaN; its gradients
     need finite ones."""
     if cu_seqlens_k is None:
@@ -197,11 +225,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     both = not causal if bidirectional is None else bool(bidirectional)
     edges = () if bias_table is None else bucket_edges(bias_table.shape[0], int(max_distance), both)
     if out is not None:
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias_table, out)):
-            raise RuntimeError("packed_attention: out= has no gradient (call it under torch.no_grad())")
-        if out.shape != q.shape or out.dtype != q.dtype or (out.numel() and _ready(out) is not out):
-            raise ValueError(f"packed_attention: out {tuple(out.shape)} {out.dtype} with strides {out.stride()} does not "
-                             f"match q {tuple(q.shape)} {q.dtype} in rows of 16-byte pieces")
+        _check_out(q, k, v, cu_seqlens_q, cu_seqlens_k, bias_table, out)
+        torch.autograd.graph.increment_version(out)
         return _forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, scale, bias_table, edges, both, out, False)[0]
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                          (bias_table is not None and bias_table.requires_grad))):

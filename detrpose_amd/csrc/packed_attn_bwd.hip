@@ -577,7 +577,7 @@ extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
   a.ktiles = p.ktiles;
   a.cuts = p.cuts;
   a.cut_tiles = p.cut_tiles;
-  DP_REQUIRE((int64_t)p.ktiles * a.hkv < INT32_MAX, "dp_packed_attn_bwd: too many tiles");
+  DP_REQUIRE(std::max<int64_t>(p.items, p.ktiles) * a.hkv <= UINT32_MAX / NT, "dp_packed_attn_bwd: too many tiles");
   a.dsum = (float*)d->ws;
   a.dbias_part = a.dsum + (int64_t)d->tq * d->heads;
   a.kv_part = a.dsum + ((int64_t)d->tq * d->heads + (a.bias ? (int64_t)p.items * d->heads * d->buckets : 0) + 3) / 4 * 4;

@@ -5,8 +5,8 @@
 // double-buffered in LDS. Per wave and 32 keys: S^T = K Q^T, p = exp(s - m), O^T += V^T P^T; a lane
 // holds one row's scores, so the maximum needs one exchange between the wave's halves, and the sum
 // none until the end. m moves only when a row's maximum grows by more than 8 in the exponent of 2
-// (p stays below 256): the rescaling of O is then rare. p is rounded to bf16 for its product (2^-9
-// rms relative, as the output's own rounding); the sum takes it unrounded.
+// (p stays below 256): the rescaling of O is then rare. p is rounded to bf16 for its product (by at most 2^-8
+// of itself, as the output's own rounding); the sum takes it unrounded.
 #include "packed_attn.h"
 #include <algorithm>
 
@@ -15,19 +15,42 @@ using namespace dppa;
 
 constexpr float GROW = 8.f;   // log2 of how far p may pass 1 before m moves
 
-// A row again, key by key: only for a wave whose result holds a NaN. In the products a hidden key's
-// weight is 0, but 0 x inf or NaN (a value that causal order hides) is NaN: here hidden keys are not read.
+// A row again, key by key: only for a wave whose result holds a NaN. In the products a key that causal order
+// hides has the weight 0, but 0 x inf or NaN (its value) is NaN: here hidden keys are not read. The keys that
+// share a tile with the row's last one are at most NEAR behind it; where their values are finite, the NaN is
+// the row's own, and so it is where one of the first 64 scores is NaN, or one of their values in every column:
+// those rows stay as they are, which keeps a model whose numbers went NaN from walking every key twice.
+constexpr int NEAR = 160;   // the wave's 32 rows, the tile's 128 keys
+
 template <typename T, typename BIASOF>
-__device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos, int q0, int k0, int lim, BIASOF bias) {
+__device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos, int q0, int k0, int lk, int lim,
+                                         BIASOF bias) {
   const int lane = threadIdx.x & 63;
   const int head = kvh * a.group + g;
   const T* q = (const T*)a.q + (int64_t)(q0 + pos) * a.q_row + head * a.q_head;
+  auto value = [&](int j, int d) {
+    return d < a.dim ? to_f32(((const T*)a.v + (int64_t)(k0 + j) * a.v_row + kvh * a.v_head)[d]) : 0.f;
+  };
+  bool hides = false;
+  for (int j = lim; j < min(lk, lim + NEAR); ++j) {
+    const float x = value(j, lane), y = value(j, lane + 64);
+    hides |= x - x != 0.f || y - y != 0.f;
+  }
+  if (!__ballot(hides)) return;
   auto score = [&](int j) {
     const T* k = (const T*)a.k + (int64_t)(k0 + j) * a.k_row + kvh * a.k_head;
     float s = 0.f;
     for (int d = 0; d < a.dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
     return s * a.scale + bias(j);
   };
+  bool n0 = lane >= a.dim, n1 = lane + 64 >= a.dim;
+  for (int j = 0; j < min(lim, 64); ++j) {
+    const float x = value(j, lane), y = value(j, lane + 64);
+    n0 |= x != x;
+    n1 |= y != y;
+  }
+  const float s0 = lane < lim ? score(lane) : 0.f;
+  if (__ballot(s0 != s0) || __ballot(n0 && n1) == ~0ull) return;
   float m = -INFINITY;
   for (int j = lane; j < lim; j += 64) m = fmaxf(m, score(j));
   m = wave_max(m);
@@ -38,9 +61,8 @@ __device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos,
     sum += p;
     for (int u = 0; u < min(64, lim - j0); ++u) {
       const float w = __shfl(p, u, 64);
-      const T* v = (const T*)a.v + (int64_t)(k0 + j0 + u) * a.v_row + kvh * a.v_head;
-      if (lane < a.dim) o0 = fmaf(w, to_f32(v[lane]), o0);
-      if (lane + 64 < a.dim) o1 = fmaf(w, to_f32(v[lane + 64]), o1);
+      o0 = fmaf(w, value(j0 + u, lane), o0);
+      o1 = fmaf(w, value(j0 + u, lane + 64), o1);
     }
   }
   sum = wave_sum(sum);
@@ -58,7 +80,7 @@ __device__ __forceinline__ void slow_row(const Args& a, int kvh, int g, int pos,
 
 // chunks that a sequence's keys are cut into, for a tile of `rows` rows
 __device__ __forceinline__ int splits_of(const Args& a, int lk, int rows) {
-  return a.splits <= 1 ? 1 : clampi((lk + a.chunk - 1) / max(a.chunk, 16 * rows), 1, a.splits);
+  return a.splits <= 1 ? 1 : clampi((int)(((unsigned)lk + a.chunk - 1) / max(a.chunk, 16 * rows)), 1, a.splits);
 }
 
 // WK waves of a block share its rows and walk the key tile's subtiles in turn; 4 / WK of them, 32 rows
@@ -248,7 +270,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
     for (unsigned left = (unsigned)redo; left; left &= left - 1) {
       const int row = first + __builtin_ctz(left), rp = row / a.group;
       const int hd = row - rp * a.group;
-      slow_row<T>(a, kvh, hd, rp, q0, k0, limit(row), [&](int j) {
+      slow_row<T>(a, kvh, hd, rp, q0, k0, lk, limit(row), [&](int j) {
         return BIAS ? bias.tab[hd * bias.nb + bias.bucket(j - rp - off)] : 0.f;
       });
     }
@@ -307,7 +329,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
       if (!redo[jr]) continue;
       const int row = row0 + jr, rp = row / a.group;
       const int hd = row - rp * a.group;
-      slow_row<T>(a, kvh, hd, rp, q0, k0, limit(row), [&](int j) {
+      slow_row<T>(a, kvh, hd, rp, q0, k0, lk, limit(row), [&](int j) {
         return BIAS ? bias.tab[hd * bias.nb + bias.bucket(j - rp - off)] : 0.f;
       });
     }
@@ -322,7 +344,7 @@ __device__ __forceinline__ void redo_row(const Args& a, int row, int head) {
   if (b == a.nseq) return;
   const int2 qs = seq_at(a.cu_q, a.nseq, a.tq, b), ks = seq_at(a.cu_k, a.nseq, a.tk, b);
   const int pos = row - qs.x, off = ks.y - qs.y;
-  slow_row<T>(a, head / a.group, head % a.group, pos, qs.x, ks.x, a.causal ? clampi(pos + off + 1, 0, ks.y) : ks.y,
+  slow_row<T>(a, head / a.group, head % a.group, pos, qs.x, ks.x, ks.y, a.causal ? clampi(pos + off + 1, 0, ks.y) : ks.y,
               [&](int j) {
                 if (!a.bias) return 0.f;
                 const int rel = j - pos - off, n = a.both ? abs(rel) : max(-rel, 0);
@@ -539,13 +561,10 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
   a->v_row = d->v_row; a->v_head = d->v_head; a->o_row = d->o_row; a->o_head = d->o_head;
   a->cu_q = d->cu_q; a->cu_k = d->cu_k; a->nseq = d->nseq; a->tq = d->tq; a->tk = d->tk;
   a->hkv = d->kv_heads; a->group = d->heads / d->kv_heads; a->dim = d->dim; a->causal = d->causal; a->scale = d->scale;
-  const int64_t tiles = (int64_t)d->tq * a->group / BM + d->nseq + 1;
-  DP_REQUIRE(tiles * a->hkv < INT32_MAX, "%s: too many tiles", what);
-  a->tiles = (int)tiles;
   if (d->bias) {
     const int nb = d->both ? d->buckets / 2 : d->buckets;
     DP_REQUIRE(d->bias_dtype == DP_F32 || d->bias_dtype == d->dtype, "%s: bias dtype %d", what, d->bias_dtype);
-    DP_REQUIRE(d->buckets >= 2 && d->buckets <= 64 && (!d->both || d->buckets % 2 == 0) && nb >= 1, "%s: %d buckets",
+    DP_REQUIRE(d->buckets >= 2 && d->buckets <= 64 && (!d->both || d->buckets % 2 == 0) && nb >= 2, "%s: %d buckets",
                what, d->buckets);
     DP_REQUIRE(a->group * d->buckets <= 4096, "%s: %d heads a group x %d buckets", what, a->group, d->buckets);
     a->bias = d->bias; a->bias_f32 = d->bias_dtype == DP_F32; a->buckets = d->buckets; a->both = d->both != 0;
@@ -567,7 +586,7 @@ extern "C" int dp_packed_attn_fwd(const dp_packed_attn* d, void* stream) {
   DP_REQUIRE(d->ws_bytes >= need && (d->ws || !need), "dp_packed_attn_fwd: workspace holds %lld bytes, needs %lld",
              (long long)d->ws_bytes, (long long)need);
   const Plan p = plan_of(d);
-  DP_REQUIRE((int64_t)p.items * a.hkv < INT32_MAX, "dp_packed_attn_fwd: too many tiles");
+  DP_REQUIRE((int64_t)p.items * a.hkv <= UINT32_MAX / NT, "dp_packed_attn_fwd: too many tiles");   // a grid's threads
   a.tiles = p.items;
   a.chunk = p.chunk;
   a.splits = p.splits;

@@ -540,3 +540,103 @@ def test_only_some_gradients():
     assert torch.equal(torch.autograd.grad(out, v, dout)[0], full["dv"])
     with torch.no_grad():
         assert not A.packed_attention(q, k, v, _cu(ql), bias_table=t).requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_strides_of_dimensions_of_one(dtype):
+    """One row or one head: whatever stride that dimension has, the rows are read and written."""
+    e = 16 // torch.empty(0, dtype=dtype).element_size()
+    base = torch.randn(1 << 16, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    row = lambda h: base.as_strided((1, h, 32), (3 * e + 1, 32, 1))  # noqa: E731
+    head = lambda n: base.as_strided((n, 1, 32), (64, 5, 1), 64 * e)  # noqa: E731
+    far = base.as_strided((1, 2, 32), (1 << 30, 32, 1))
+    for q, k in ((row(4), row(2)), (head(50), head(50)), (far, far)):
+        lens = [q.shape[0]]
+        dout = torch.ones_like(q)
+        got, want = _run(q, k, k, dout, lens, lens), _run(q.clone(), k.clone(), k.clone(), dout, lens, lens)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+        out = torch.zeros(1 << 16, device="cuda", dtype=dtype).as_strided(q.shape, q.stride())
+        with torch.no_grad():
+            A.packed_attention(q, k, k, _cu(lens), out=out)
+        assert torch.equal(out, want["out"])
+
+
+@pytest.mark.gpu
+def test_out_apart_from_what_is_read():
+    """out= across an input, or across itself, is refused; a tensor that autograd holds is known as changed."""
+    q, k, v, _, _ = _inputs(13, torch.float32, 2, 2, 32, [6], [6])
+    cu = _cu([6])
+    for bad in (q, k, v):
+        with pytest.raises(ValueError, match="lies across"):
+            A.packed_attention(q, k, v, cu, out=bad)
+    with pytest.raises(ValueError, match="lies across k"):
+        both = torch.zeros(6, 4, 32, device="cuda")
+        A.packed_attention(q, both[:, :2], v, cu, out=both[:, 2:])
+    flat = torch.zeros(4096, device="cuda")
+    for strides in ((0, 32, 1), (64, 0, 1), (32, 32, 1), (64, 16, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            A.packed_attention(q, k, v, cu, out=flat.as_strided((6, 2, 32), strides))
+    want = A.packed_attention(q, k, v, cu)
+    for strides in ((32, 192, 1), (128, 32, 1), (64, 32, 1)):   # head first, gaps, plain
+        assert torch.equal(A.packed_attention(q, k, v, cu, out=flat.as_strided((6, 2, 32), strides)), want)
+    x = torch.ones(6, 2, 32, device="cuda", requires_grad=True)
+    out = torch.ones(6, 2, 32, device="cuda")
+    y = (x * out).sum()
+    A.packed_attention(q, k, v, cu, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
+def test_two_way_buckets_need_two_a_direction():
+    import ctypes as C
+    from detrpose_amd import _lib
+    a = _lib.PackedAttn()
+    for n in ("q", "k", "v", "out", "cu_q", "cu_k", "bias"):
+        setattr(a, n, 4096)   # never dereferenced
+    for n in ("q", "k", "v", "o"):
+        setattr(a, n + "_row", 64)
+        setattr(a, n + "_head", 32)
+    a.nseq, a.tq, a.tk, a.heads, a.kv_heads, a.dim, a.scale, a.dtype = 1, 4, 4, 2, 2, 32, 1.0, 1
+    a.buckets, a.both = 2, 1
+    assert _lib.load().dp_packed_attn_fwd(C.byref(a), None) == 1000
+    # more blocks than a grid takes threads for
+    a.bias, a.nseq, a.tq, a.tk, a.heads, a.kv_heads = None, 1 << 24, 1 << 24, 1 << 24, 2, 2
+    a.ws_bytes, a.ws = 1 << 60, 4096
+    assert _lib.load().dp_packed_attn_fwd(C.byref(a), None) == 1000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[150], [1, 300], [40, 2100]], ids=str)
+def test_where_nan_is_seen(dtype, lens):
+    """NaN or inf in q, k, v: exactly the outputs that see one are not finite, however many rows do."""
+    n = sum(lens)
+    for case in ("q", "k", "v", "all", "column", "late"):
+        q, k, v, _, _ = _inputs(14, dtype, 2, 1, 64, lens, lens)
+        want = torch.zeros(n, 2, 64, dtype=torch.bool, device="cuda")
+        s0 = n - lens[-1]
+        if case == "q":
+            q[n - 5, 1] = float("nan")
+            want[n - 5, 1] = True
+        elif case == "k":
+            k[s0] = float("nan")
+            want[s0:] = True
+        elif case == "v":
+            v[n - 30] = float("inf")
+            want[n - 30:] = True
+        elif case == "all":
+            q[:], k[:], v[:] = (float("nan"),) * 3
+            want[:] = True
+        elif case == "column":
+            v[:, :, 9] = float("nan")
+            want[:, :, 9] = True
+        else:
+            v[s0 + 100:, :, 3] = float("nan")
+            k[s0 + 120:] = float("inf")
+            want[s0 + 100:, :, 3] = True
+            want[s0 + 120:] = True
+        got = A.packed_attention(q, k, v, _cu(lens), causal=True)
+        if case == "late":   # q k is inf or NaN by its signs: -inf hides the key again
+            got, want = got[:s0 + 120], want[:s0 + 120]
+        assert torch.equal(~torch.isfinite(got), want), case
