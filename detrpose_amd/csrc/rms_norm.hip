@@ -170,9 +170,10 @@ __global__ __launch_bounds__(threads<TPR>()) void rms_fwd_kernel(void* __restric
     if (!E4M3) row_store<T, N>((T*)yv + (int64_t)row * c, t + TPR * i, c, a[i]);
   }
   if constexpr (E4M3) {
-    // scale = max |y| / 448; a row of zeros gets scale 0 and zeros (its values stand for 0 x 0)
+    // scale = max |y| / 448; a row of zeros gets scale 0 and zeros (its values stand for 0 x 0). Below the
+    // normal numbers the quotient rounds so far that max |y| / scale passes 448, which e4m3 has no number for
     top = row_reduce<TPR, true>(top, red[1]);
-    const float sc = top / 448.f;
+    const float sc = top > 0.f ? fmaxf(top / 448.f, 0x1p-126f) : 0.f;
     if (t == 0) scale[row] = sc;
     uint8_t* yp = (uint8_t*)yv + (int64_t)row * c;
 #pragma unroll
@@ -336,10 +337,16 @@ struct FwdArgs {
 
 template <typename T, typename W, int TPR, int V, bool E4M3>
 void fwd_launch(const FwdArgs& a) {
-  const int rpb = threads<TPR>() / TPR;
-  hipLaunchKernelGGL((rms_fwd_kernel<T, W, TPR, V, E4M3>), dim3((a.rows + rpb - 1) / rpb), dim3(threads<TPR>()), 0, a.s, a.y,
-                     a.scale, (T*)a.r, a.rstd, (const T*)a.x, a.ld_x, (const T*)a.res, a.ld_res, (const W*)a.w, a.eps,
-                     a.rows, a.c);
+  constexpr int rpb = threads<TPR>() / TPR;
+  constexpr int most = (int)(UINT32_MAX / threads<TPR>()) * rpb;   // rows of a launch: a grid has less than 2^32 threads
+  for (int64_t r0 = 0; r0 < a.rows; r0 += most) {
+    const int rows = (int)std::min<int64_t>(most, a.rows - r0);
+    hipLaunchKernelGGL((rms_fwd_kernel<T, W, TPR, V, E4M3>), dim3((rows + rpb - 1) / rpb), dim3(threads<TPR>()), 0, a.s,
+                       (char*)a.y + r0 * a.c * (E4M3 ? 1 : sizeof(T)), a.scale ? a.scale + r0 : nullptr,
+                       a.r ? (T*)a.r + r0 * a.c : nullptr, a.rstd ? a.rstd + r0 : nullptr, (const T*)a.x + r0 * a.ld_x,
+                       a.ld_x, a.res ? (const T*)a.res + r0 * a.ld_res : nullptr, a.ld_res, (const W*)a.w, a.eps, rows,
+                       a.c);
+  }
 }
 
 template <typename T, typename W, bool E4M3>

@@ -224,3 +224,52 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for a, b in zip(outs, step(x, w, dy)):
             assert torch.equal(a, b), k
+
+
+@pytest.mark.gpu
+def test_e4m3_rows_below_the_normal_numbers():
+    """A norm whose 448th part is no normal f32 keeps finite values: the scale stays at 2^-126, and a value is off
+    by at most half the least step 2^-10 of it or 2^-4 of itself, and the f32 product's half step 2^-150."""
+    x = torch.randn(6, 300, generator=torch.Generator().manual_seed(4)).cuda()
+    for tiny in (1e-36, 1e-38, 1e-40, 1e-42, 1e-44):
+        w = torch.full((300,), tiny, device="cuda")
+        y, s, _ = N.rms_norm_e4m3(x, w, eps=EPS)
+        assert torch.isfinite(y.float()).all() and (s >= 2.0 ** -126).all()
+        y0 = x.double() * (x.double().pow(2).mean(-1, keepdim=True) + EPS).rsqrt() * w.double()
+        err = (y.double() * s.double()[:, None] - y0).abs()
+        lim = (2.0 ** -4 + 310 * 2.0 ** -24) * y0.abs() + 2.0 ** -10 * s.double()[:, None] + 2.0 ** -149
+        assert (err <= lim).all(), tiny
+
+
+@pytest.mark.gpu
+def test_same_tensor_twice_and_modes():
+    """x as its own residual, with gradients from both uses; no graph in no_grad and inference_mode."""
+    x = torch.randn(5, 64, generator=torch.Generator().manual_seed(5)).cuda().requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    y, r = N.rms_norm(x, w, residual=x)
+    assert torch.equal(r, 2 * x)
+    gx, gw = torch.autograd.grad(y.sum() + r.sum(), [x, w])
+    x2 = x.detach().clone().requires_grad_()
+    y2, r2 = N.rms_norm(2 * x2, w, residual=torch.zeros_like(x2))
+    gx2, gw2 = torch.autograd.grad(y2.sum() + r2.sum(), [x2, w])
+    assert torch.equal(gx, gx2) and torch.equal(gw, gw2)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            y3, r3 = N.rms_norm(x, w, residual=x)
+            y8, s8, r8 = N.rms_norm_e4m3(x, w, residual=x)
+        assert torch.equal(y3, y) and not y3.requires_grad and torch.equal(r8, r3)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_grid_has_threads():
+    """2^32 threads of 256 a row: the rows behind them are computed by a second launch."""
+    rows, c = (1 << 24) + 5, 1032
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("80 GiB of memory")
+    x = torch.zeros(rows, c, device="cuda", dtype=torch.bfloat16)
+    x[-9:] = torch.randn(9, c, generator=torch.Generator().manual_seed(6)).bfloat16()
+    x[0] = x[-1]
+    w = torch.linspace(0.5, 2, c, device="cuda")
+    y = N.rms_norm(x, w)
+    assert torch.equal(y[-9:], N.rms_norm(x[-9:].clone(), w)) and torch.equal(y[0], y[-1])
+    assert not y[1000].any() and not y[-10].any()
