@@ -95,4 +95,5 @@ def clip_grad_norm_(parameters, max_norm, out=None):
                                     0 if out is None else out.numel(),
                                     _lib.DP_F32 if out is None else _DT[out.dtype], ws.data_ptr(), nb,
                                     C.c_void_p(s)), "dp_grad_clip")
+    torch.autograd.graph.increment_version(grads if out is None else [out])
     return norm

@@ -169,3 +169,15 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         other = torch.empty_like(out)
         assert torch.equal(G.clip_grad_norm_(grads, 1.0, out=other), norm) and torch.equal(out, other), k
+
+
+@pytest.mark.gpu
+def test_autograd_sees_what_was_written():
+    """Tensors that a graph holds are known as changed, clipped in place or gathered into."""
+    x = torch.ones(9, device="cuda", requires_grad=True)
+    for out in (None, torch.ones(9, device="cuda")):
+        g = torch.ones(9, device="cuda")
+        y = (x * (g if out is None else out)).sum()
+        G.clip_grad_norm_([g], 0.5, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
