@@ -119,8 +119,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
 def rms_norm_e4m3(x, weight, residual=None, eps=1e-6):
     """The same norm with an 8-bit output, for serving: (y, scale, r) with y (..., c) float8_e4m3fn and
-    scale (...) f32, y * scale[..., None] standing for the norm: scale = max |norm| / 448 of its row (a row of
-    zeros has scale 0). r = x + residual, or None without a residual. Has no gradient."""
+    scale (...) f32, y * scale[..., None] standing for the norm: scale = max |norm| / 448 of its row, 2^-126 at
+    least (a row of zeros has scale 0). r = x + residual, or None without a residual. Has no gradient."""
     _check("rms_norm_e4m3", x, weight, residual, eps)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_e4m3: the 8-bit form has no gradient (use rms_norm, or torch.no_grad())")

@@ -750,7 +750,8 @@ int dp_maxpool2x2_pad_rb_bwd(const void* x, int64_t x_bstride, int32_t x_pstride
  *  bias: NULL or a learned table [buckets][heads] (f32, or dtype): the bias of pair (i, j) is
  *  bias[bucket(j - position)][h]. n = |j - position| (one direction: max(position - j, 0)) falls into
  *  the bucket numbered by how many of edge[0 .. nb - 2] are <= n, nb = buckets (both directions: half of
- *  them, and keys behind the query's position take the other half). edge: from 1, not falling, the last <= 4096.
+ *  them, and keys behind the query's position take the other half); nb at least 2. edge: from 1, not
+ *  falling, the last <= 4096.
  *  fill_tail: rows of out behind the last sequence are written as zeros (else left as they are).
  *  ws: dp_packed_attn_ws_bytes(desc, 0) bytes. */
 typedef struct dp_packed_attn {
@@ -785,7 +786,8 @@ int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream);
  * 16384 (bf16); rows need only their element's alignment. */
 int dp_rms_norm(void* y, void* r, float* rstd, const void* x, int64_t ld_x, const void* res, int64_t ld_res,
                 const void* weight, int32_t w_dtype, float eps, int32_t rows, int32_t c, int32_t dtype, void* stream);
-/* The same with an 8-bit output: y e4m3 [rows][c] = norm / scale, scale f32 [rows] = max |norm| / 448. */
+/* The same with an 8-bit output: y e4m3 [rows][c] = norm / scale, scale f32 [rows] = max |norm| / 448 (2^-126 at
+ * least; 0 for a row of zeros). */
 int dp_rms_norm_e4m3(void* y, float* scale, void* r, const void* x, int64_t ld_x, const void* res, int64_t ld_res,
                      const void* weight, int32_t w_dtype, float eps, int32_t rows, int32_t c, int32_t dtype,
                      void* stream);
