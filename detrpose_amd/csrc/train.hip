@@ -89,12 +89,13 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(T* __restrict__ dx, const T
       const int j = lane + 64 * t;
       xh[t] = gy[t] = d[t] = 0.f;
       if (j < c) {
+#pragma clang fp contract(off)   // products rounded before they are added, but where fmaf says otherwise
         d[t] = to_f32(dy[(int64_t)r * ld_dy + j]);
         xh[t] = (to_f32(s[(int64_t)r * c + j]) - mean) * rstd;
         gy[t] = d[t] * g[j];
         s1 += gy[t];
         s2 += gy[t] * xh[t];
-        pg[t] += d[t] * xh[t];
+        pg[t] = fmaf(d[t], xh[t], pg[t]);
         pb[t] += d[t];
       }
     }
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(T* __restrict__ dx, const T
     for (int t = 0; t < LN_E; ++t) {
       const int j = lane + 64 * t;
       if (j < c) {
-        float o = rstd * (gy[t] - s1 - xh[t] * s2);
+        float o = rstd * fmaf(-s2, xh[t], gy[t] - s1);
         T* p = dx + (int64_t)r * c + j;
         if (acc) o += to_f32(*p);
         *p = from_f32<T>(o);
@@ -169,10 +170,16 @@ __global__ __launch_bounds__(256) void ln_fwd_vec_kernel(T* __restrict__ y, int 
   float sum = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) sum += v[e];
-  const float mean = wave_sum(sum) / c;
-  float q = 0.f;
+  float mean, q = 0.f;
+  {
+#pragma clang fp contract(off)   // the mean and the squares are rounded before they go on, whatever the compiler fuses
+    mean = wave_sum(sum) / c;
 #pragma unroll
-  for (int e = 0; e < E; ++e) q += (v[e] - mean) * (v[e] - mean);
+    for (int e = 0; e < E; ++e) {
+      v[e] = v[e] - mean;
+      q += v[e] * v[e];
+    }
+  }
   const float rstd = rsqrtf(wave_sum(q) / c + eps);
   if (lane == 0) {
     stats[2 * (int64_t)r] = mean;
@@ -189,7 +196,7 @@ __global__ __launch_bounds__(256) void ln_fwd_vec_kernel(T* __restrict__ y, int 
   }
   float o[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = (v[e] - mean) * rstd * g[j0 + e] + bt[j0 + e] + (addp ? pv[e] : 0.f);
+  for (int e = 0; e < E; ++e) o[e] = v[e] * rstd * g[j0 + e] + bt[j0 + e] + (addp ? pv[e] : 0.f);
   stE<T, E>(y + (int64_t)r * ld_y + j0, o);
 }
 
@@ -207,24 +214,25 @@ __global__ __launch_bounds__(256) void ln_bwd_vec_kernel(T* __restrict__ dx, con
   for (int e = 0; e < E; ++e) gw[e] = g[j0 + e], pg[e] = pb[e] = 0.f;
   for (int r = blockIdx.x * 4 + wave; r < rows; r += gridDim.x * 4) {
     const float mean = stats[2 * (int64_t)r], rstd = stats[2 * (int64_t)r + 1];
-    float d[E], xh[E], gy[E];
+    float d[E], xh[E];
     ldE<T, E>(dy + (int64_t)r * ld_dy + j0, d);
     ldE<T, E>(s + (int64_t)r * c + j0, xh);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+#pragma clang fp contract(off)   // products rounded before they are added, but where fmaf says otherwise
       xh[e] = (xh[e] - mean) * rstd;
-      gy[e] = d[e] * gw[e];
-      s1 += gy[e];
-      s2 += gy[e] * xh[e];
-      pg[e] += d[e] * xh[e];
+      const float gy = d[e] * gw[e];
+      s1 += gy;
+      s2 += gy * xh[e];
+      pg[e] = fmaf(d[e], xh[e], pg[e]);
       pb[e] += d[e];
     }
     s1 = wave_sum(s1) / c;
     s2 = wave_sum(s2) / c;
     float o[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = rstd * (gy[e] - s1 - xh[e] * s2);
+    for (int e = 0; e < E; ++e) o[e] = rstd * fmaf(-s2, xh[e], fmaf(d[e], gw[e], -s1));
     T* p = dx + (int64_t)r * c + j0;
     if (acc) {
       float pr[E];
@@ -581,7 +589,13 @@ __global__ void gate_fwd_kernel(const T* __restrict__ G, const T* __restrict__ x
     const float g1 = sigmoidf_(to_f32(G[b2 + j])), g2 = sigmoidf_(to_f32(G[b2 + c + j]));
     gs[b2 + j] = from_f32<T>(g1);
     gs[b2 + c + j] = from_f32<T>(g2);
-    z[e] = from_f32<T>(g1 * to_f32(xcat[b2 + j]) + g2 * to_f32(xcat[b2 + c + j]));
+    const float x1 = to_f32(xcat[b2 + j]), x2 = to_f32(xcat[b2 + c + j]);
+    if constexpr (sizeof(T) == 4) {
+#pragma clang fp contract(off)   // f32: both products rounded alike
+      z[e] = g1 * x1 + g2 * x2;
+    } else {
+      z[e] = from_f32<T>(g1 * x1 + g2 * x2);
+    }
   }
 }
 
@@ -713,7 +727,10 @@ __global__ void pose_refine_bwd_kernel(const float* __restrict__ corners, const 
   for (int i = 0; i < nb; ++i) {
     const float p = __expf(cr[i] - mx);
     den += p;
-    num += p * proj[i];
+    {
+#pragma clang fp contract(off)
+      num += p * proj[i];
+    }
   }
   const float mean_w = num / den;
   const float g = dk[e] * inv_s;
@@ -928,11 +945,15 @@ __global__ void cdn_build_kernel(const int* __restrict__ off, const int* __restr
     // direction: normalize(rand_like) (first quadrant, dn_component.py:121-122); distance:
     // alpha ~ U(0, ln 2) positive / U(ln 2, ln 10) negative, * 2 (area*h*w + eps) var, sqrt, / max(h, w)
     const float u1 = urand(seed, 3, key + pt), u2 = urand(seed, 4, key + pt);
-    const float nrm = fmaxf(sqrtf(u1 * u1 + u2 * u2), 1e-12f);
     const float ua = urand(seed, 5, key + pt);
     const bool neg = g & 1;
     const float lo = neg ? 0.69314718f : 0.f, hi = neg ? 2.30258509f : 0.69314718f;
-    float alpha = lo + (hi - lo) * ua;
+    float nrm, alpha;
+    {
+#pragma clang fp contract(off)   // equal draws give equal noise, whatever the compiler fuses
+      nrm = fmaxf(sqrtf(u1 * u1 + u2 * u2), 1e-12f);
+      alpha = lo + (hi - lo) * ua;
+    }
     const float s2 = 2.f * sig[pt];
     alpha *= 2.f * (area[tg] * img_h * img_w + 1.1920929e-07f) * s2 * s2;
     alpha = sqrtf(alpha) / fmaxf(img_h, img_w);
@@ -993,13 +1014,15 @@ __global__ void adamw_kernel(float* __restrict__ p, const float* __restrict__ g,
     scale = fminf(max_norm / (nrm + 1e-6f), 1.f);
   }
   const float gi = g[i] * scale;
-  float pi = p[i] * (1.f - lr * wd);
+  const float keep = 1.f - lr * wd;
   const float mi = b1 * m[i] + (1.f - b1) * gi;
-  const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
   m[i] = mi;
-  v[i] = vi;
-  pi -= (lr / bc1) * mi / (sqrtf(vi) / sqrtf(bc2) + eps);
-  p[i] = pi;
+  {
+#pragma clang fp contract(off)   // equal states give equal updates, whatever the compiler fuses
+    const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
+    v[i] = vi;
+    p[i] = p[i] * keep - (lr / bc1) * mi / (sqrtf(vi) / sqrtf(bc2) + eps);
+  }
 }
 
 // bad[0] = 1 when any of v[0..n) is not finite (left unchanged otherwise): one block
@@ -1014,7 +1037,10 @@ __global__ void ema_kernel(float* __restrict__ e, const float* __restrict__ p, i
                            const float* __restrict__ skip) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n || (skip && *skip != 0.f)) return;
-  e[i] = d * e[i] + (1.f - d) * p[i];
+  {
+#pragma clang fp contract(off)   // both products rounded alike
+    e[i] = d * e[i] + (1.f - d) * p[i];
+  }
 }
 
 inline unsigned nblk(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
