@@ -37,6 +37,9 @@ constexpr float LN2 = 0.69314718055994530942f;
 constexpr int NT = 256;     // threads of a block: 4 waves, 32 rows (or keys) each
 constexpr int BM = 128;     // rows (keys, in the dk / dv kernel) of a block
 
+// dk / dv: a run [w0, w1) of a key tile's walk over the queries; row: where its part goes, if there are several
+struct alignas(16) Piece { int start, len, start2, len2, tile, w0, w1, parts, begins, row, unused[2]; };
+
 // what a kernel needs to know; strides in elements
 struct Args {
   const void *q, *k, *v;
@@ -61,9 +64,11 @@ struct Args {
   void *dq, *dk, *dv;
   float* dsum;
   float* dbias_part;
-  int ktiles, cut_tiles, cuts;   // dk / dv: blocks, query tiles of a cut, most cuts of one sequence
+  // dk / dv, of one key head: blocks, units of a share at least, places for parts, shares and pieces at most
+  int kblocks, kunits, kslots, kshares, kpieces;
   float* kv_part;
-  int* kv_n;
+  int2 *kv_n, *kv_share;
+  Piece* kv_piece;
 };
 
 // A wave-uniform value in a scalar register (the empty asm keeps it there: the compiler drops a

@@ -640,3 +640,38 @@ def test_where_nan_is_seen(dtype, lens):
         if case == "late":   # q k is inf or NaN by its signs: -inf hides the key again
             got, want = got[:s0 + 120], want[:s0 + 120]
         assert torch.equal(~torch.isfinite(got), want), case
+
+
+# dk and dv in shares that begin and end anywhere in a tile's walk: many key heads, so few shares a head
+SHARES = [
+    (32, 32, 32, [700, 1, 260, 0, 90], None, True, 0),
+    (32, 32, 128, [400, 33, 129], None, True, 0),
+    (64, 32, 64, [300, 7, 500], [500, 0, 400], True, 8),       # queries over more, no and fewer keys
+    (32, 32, 64, [257, 100], [130, 513], False, 0),
+    (64, 64, 16, [(i * 37) % 90 for i in range(150)], None, True, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHARES, ids=lambda s: f"h{s[0]}k{s[1]}d{s[2]}n{len(s[3])}b{s[6]}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_shares(shape, dtype):
+    heads, hk, d, ql, kl, causal, nb = shape
+    kl = kl or ql
+    q, k, v, dout, t = _inputs(d + nb + len(ql), dtype, heads, hk, d, ql, kl, nb, extra=140)
+    got = _run(q, k, v, dout, ql, kl, t, causal=causal)
+    want = _reference(q, k, v, ql, kl, causal, d ** -0.5, t, 128, not causal, dout)
+    for n in want:
+        _check(got[n], want[n], n)
+    again = _run(q, k, v, dout, ql, kl, t, causal=causal)
+    assert all(torch.equal(again[n], got[n]) for n in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nb", [0, 8])
+def test_no_queries_or_no_keys(nb):
+    for n, m in ((0, 150), (150, 0), (0, 0)):
+        q, k, v, dout, t = _inputs(15, torch.bfloat16, 4, 2, 64, [n], [m], nb)
+        got = _run(q, k, v, dout, [n], [m], t, causal=True)
+        assert got["out"].shape == q.shape and got["dk"].shape == k.shape
+        assert all(not x.any() for x in got.values())
