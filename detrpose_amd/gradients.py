@@ -29,12 +29,19 @@ def _dense(t):
     return True
 
 
+def _holds(t):
+    """Whether a tensor stands for its .grad: a parameter, frozen or not, and every leaf that has or asks for one."""
+    return isinstance(t, torch.nn.Parameter) or (t.is_leaf and (t.requires_grad or t.grad is not None))
+
+
 def clip_grad_norm_(parameters, max_norm, out=None):
     """Clip gradients by their global 2-norm: g * min(1, max_norm / (norm + 1e-6)) for every tensor.
 
-    parameters: a tensor or an iterable of tensors. A leaf that requires a gradient stands for its .grad
-    (and is passed over while that is None); any other tensor is itself a gradient. Gradients are f32
-    or bf16, mixed as they come, all on one GPU; no two of them share memory.
+    parameters: a tensor or an iterable of tensors, either parameters or gradients. A torch.nn.Parameter, frozen
+    or not, and a leaf that requires a gradient or has one stand for their .grad, and are passed over while
+    that is None; other tensors are gradients themselves. Both kinds in one call are refused: a frozen weight that
+    is a plain tensor could not be told from a gradient. Gradients are f32 or bf16, mixed as they come, all
+    on one GPU; no two of them share memory.
     out: None clips in place. A contiguous 1-d f32 or bf16 tensor of as many elements as the
     gradients together takes the clipped gradients one behind the other, in their order, and the
     gradients are left as they are.
@@ -46,8 +53,15 @@ def clip_grad_norm_(parameters, max_norm, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
-    grads = [p.grad if p.requires_grad and p.is_leaf else p for p in parameters]
-    grads = [g for g in grads if g is not None]
+    tensors = list(parameters)
+    holds = list(map(_holds, tensors))
+    if any(holds):
+        if not all(holds):
+            raise ValueError(f"clip_grad_norm_: parameters and, at {holds.index(False)}, a tensor that neither is one nor "
+                             "requires a gradient: pass parameters or gradients")
+        grads = [g for g in (p.grad for p in tensors) if g is not None]
+    else:
+        grads = tensors
     if not grads:
         if out is not None and out.numel():
             raise ValueError(f"clip_grad_norm_: out holds {out.numel()} elements, the gradients 0")

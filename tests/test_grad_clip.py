@@ -181,3 +181,45 @@ def test_autograd_sees_what_was_written():
         G.clip_grad_norm_([g], 0.5, out=out)
         with pytest.raises(RuntimeError, match="modified by an inplace"):
             y.backward()
+
+
+def test_frozen_parameters_are_not_gradients():
+    """A parameter stands for its .grad whether it asks for one or not: without one it is passed over."""
+    from detrpose_amd import build_model
+    model, _ = build_model("n")
+    frozen = {n: p.detach().clone() for n, p in model.named_parameters() if not p.requires_grad}
+    assert {"transformer.up", "transformer.reg_scale"} <= frozen.keys()
+    assert G.clip_grad_norm_(model.parameters(), 0.1) == 0            # no gradients yet
+    assert G.clip_grad_norm_(model.parameters(), 0.1, out=torch.zeros(0)) == 0
+    assert all(torch.equal(p, frozen[n]) for n, p in model.named_parameters() if n in frozen)
+    late = torch.ones(3, requires_grad=True)                          # frozen after its backward pass
+    late.sum().backward()
+    late.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="one GPU"):                # its .grad, which is on the CPU
+        G.clip_grad_norm_([late, *model.parameters()], 0.1)
+    with pytest.raises(ValueError, match="pass parameters or gradients"):
+        G.clip_grad_norm_([*model.parameters(), torch.ones(3)], 0.1)
+
+
+@pytest.mark.gpu
+def test_frozen_parameters_of_the_model():
+    from detrpose_amd import build_model
+    model = build_model("n")[0].cuda()
+    model.backbone.requires_grad_(False)
+    kept = {n: p.detach().clone() for n, p in model.named_parameters()}
+    gen = torch.Generator("cuda").manual_seed(5)
+    trained = [p for p in model.parameters() if p.requires_grad]
+    assert 0 < len(trained) < len(kept) - 2
+    for p in trained:
+        p.grad = torch.randn(p.shape, generator=gen, device="cuda")
+    ref = [p.grad.clone() for p in trained]
+    true = _norm(ref)
+    flat = torch.empty(sum(g.numel() for g in ref), device="cuda")
+    norm = G.clip_grad_norm_(model.parameters(), 0.5 * true, out=flat)
+    assert abs(norm.item() - true) <= 1.1 * 2.0 ** -24 * true
+    _check([t.view_as(g) for t, g in zip(flat.split([g.numel() for g in ref]), ref)], ref, 0.5 * true / (true + 1e-6))
+    assert torch.equal(G.clip_grad_norm_(model.parameters(), 0.5 * true), norm)
+    _check([p.grad for p in trained], ref, 0.5 * true / (true + 1e-6))
+    for n, p in model.named_parameters():
+        assert torch.equal(p, kept[n]), n
+        assert p.requires_grad or p.grad is None, n
