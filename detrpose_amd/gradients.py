@@ -45,7 +45,8 @@ def clip_grad_norm_(parameters, max_norm, out=None):
     out: None clips in place. A contiguous 1-d f32 or bf16 tensor of as many elements as the
     gradients together takes the clipped gradients one behind the other, in their order, and the
     gradients are left as they are.
-    Returns the norm (before clipping) as an f32 scalar on the GPU: nothing waits for it. A norm that is not
+    Returns the norm (before clipping) as an f32 scalar on the GPU: nothing waits for it. Where there is no gradient
+    it is 0, on the device of out or of the first tensor (an empty list: on the CPU). A norm that is not
     finite makes the clipped gradients NaN (or 0 for finite ones under an infinite norm), as
     torch.nn.utils.clip_grad_norm_ without error_if_nonfinite. Deterministic: equal gradients give equal bits."""
     if isinstance(parameters, torch.Tensor):
@@ -65,7 +66,8 @@ def clip_grad_norm_(parameters, max_norm, out=None):
     if not grads:
         if out is not None and out.numel():
             raise ValueError(f"clip_grad_norm_: out holds {out.numel()} elements, the gradients 0")
-        return torch.zeros((), device=out.device if out is not None else None)
+        at = out if out is not None else tensors[0] if tensors else None
+        return torch.zeros((), device=None if at is None else at.device, dtype=torch.float32)
     device = grads[0].device
     kinds = {g.dtype for g in grads}
     if kinds - _DT.keys():

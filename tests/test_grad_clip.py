@@ -223,3 +223,16 @@ def test_frozen_parameters_of_the_model():
     for n, p in model.named_parameters():
         assert torch.equal(p, kept[n]), n
         assert p.requires_grad or p.grad is None, n
+
+
+def test_norm_of_no_gradients():
+    """0 as f32, on the device of the parameters that have no gradient (of out, when it is given)."""
+    torch.set_default_dtype(torch.float64)
+    try:
+        bare = [torch.nn.Parameter(torch.zeros(3, device="meta")) for _ in range(2)]
+        n = G.clip_grad_norm_(bare, 1.0)
+        assert n.device.type == "meta" and n.dtype == torch.float32 and n.shape == ()
+        assert G.clip_grad_norm_(bare, 1.0, out=torch.zeros(0)).device.type == "cpu"
+        assert G.clip_grad_norm_([], 1.0).dtype == torch.float32
+    finally:
+        torch.set_default_dtype(torch.float32)
