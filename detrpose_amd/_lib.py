@@ -271,6 +271,15 @@ def device_of(t):
     return _here if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
+def refuse_tangents(what, *tensors):
+    """The kernels compute no forward-mode derivative: an input that carries a tangent would lose it silently."""
+    from torch.autograd import forward_ad
+    if getattr(forward_ad, "_current_level", 0) < 0:   # outside forward mode no tensor has one
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivative (an input carries a tangent)")
+
+
 def check(rc: int, what: str = ""):
     if rc:
         msg = load().dp_last_error().decode(errors="replace")

@@ -209,8 +209,8 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     unless causal) keys behind the position take the upper half of the buckets, otherwise they count as
     distance 0. It differs by head, and its gradient is summed in f32.
 
-    Returns (Tq, heads, dim) of q's type; rows behind the last sequence are zeros. Differentiable (once) in q,
-    k, v and bias_table, with equal bits for equal inputs; gradients of rows behind the last sequence are
+    Returns (Tq, heads, dim) of q's type; rows behind the last sequence are zeros. Differentiable (once, in
+    reverse) in q, k, v and bias_table, with equal bits for equal inputs; gradients of rows behind the last sequence are
     zeros. Scores and sums are f32; in bf16 the weights (and their gradients) are rounded to bf16 for the
     products with v, q and k. out: the result is written here instead, rows behind the last sequence are left
     as they are; without gradients only, and in memory apart from what is read.
@@ -221,6 +221,7 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     if scale is None:
         scale = float(q.shape[-1] or 1) ** -0.5 if q.dim() == 3 else 1.0
     scale = float(scale)
+    _lib.refuse_tangents("packed_attention", q, k, v, bias_table, out)
     _check(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, bias_table, out)
     both = not causal if bidirectional is None else bool(bidirectional)
     edges = () if bias_table is None else bucket_edges(bias_table.shape[0], int(max_distance), both)

@@ -68,6 +68,7 @@ def clip_grad_norm_(parameters, max_norm, out=None):
             raise ValueError(f"clip_grad_norm_: out holds {out.numel()} elements, the gradients 0")
         at = out if out is not None else tensors[0] if tensors else None
         return torch.zeros((), device=None if at is None else at.device, dtype=torch.float32)
+    _lib.refuse_tangents("clip_grad_norm_", out, *grads)
     device = grads[0].device
     kinds = {g.dtype for g in grads}
     if kinds - _DT.keys():

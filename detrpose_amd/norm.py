@@ -19,6 +19,7 @@ _LONGEST = {torch.float32: 8192, torch.bfloat16: 16384}   # elements of a row
 
 
 def _check(name, x, weight, residual, eps):
+    _lib.refuse_tangents(name, x, weight, residual)
     if x.dtype not in _DT:
         raise TypeError(f"{name}: x dtype {x.dtype} (f32 / bf16)")
     if weight.dtype not in (torch.float32, x.dtype):
@@ -112,7 +113,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     """x (..., c) f32 / bf16, weight (c,) f32 or x's type -> y = r / sqrt(mean r^2 + eps) * weight with
     r = x, or, with a residual of x's shape and type, r = x + residual rounded to that type; then
     (y, r) is returned, r being the residual stream behind this addition. Sums and the norm are f32.
-    Rows of up to 16384 bf16 or 8192 f32 elements. Differentiable (once) in x, weight and residual."""
+    Rows of up to 16384 bf16 or 8192 f32 elements. Differentiable (once, in reverse) in x, weight
+    and residual."""
     _check("rms_norm", x, weight, residual, eps)
     return RMSNormFunction.apply(x, weight, residual, float(eps))
 

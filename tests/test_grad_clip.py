@@ -236,3 +236,14 @@ def test_norm_of_no_gradients():
         assert G.clip_grad_norm_([], 1.0).dtype == torch.float32
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+def test_forward_mode_is_refused():
+    """Gradients with a tangent are not clipped behind its back, nor gathered into a tensor with one."""
+    from torch.autograd import forward_ad
+    g = torch.ones(4)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(4), torch.ones(4))
+        for call in (lambda: G.clip_grad_norm_([g, dual], 1.0), lambda: G.clip_grad_norm_([g], 1.0, out=dual)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

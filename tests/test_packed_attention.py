@@ -675,3 +675,19 @@ def test_no_queries_or_no_keys(nb):
         got = _run(q, k, v, dout, [n], [m], t, causal=True)
         assert got["out"].shape == q.shape and got["dk"].shape == k.shape
         assert all(not x.any() for x in got.values())
+
+
+def test_forward_mode_is_refused():
+    """A tangent is never dropped: the call says that it has no forward-mode derivative."""
+    from torch.autograd import forward_ad
+    q, cu = torch.zeros(4, 2, 32), torch.tensor([0, 4], dtype=torch.int32)
+    table = torch.zeros(8, 2)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args, kw in (((dual(q), q, q), {}), ((q, dual(q), q), {}), ((q, q, dual(q)), {}),
+                         ((q, q, q), dict(bias_table=dual(table))), ((q, q, q), dict(out=dual(torch.zeros(4, 2, 32)))),
+                         ((dual(q), q, q), dict(out=torch.zeros(4, 2, 32)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.packed_attention(*args, cu, **kw)
+        with pytest.raises(RuntimeError, match="on the GPU"):   # none of them has a tangent
+            A.packed_attention(q, q, q, cu)

@@ -273,3 +273,15 @@ def test_more_rows_than_a_grid_has_threads():
     y = N.rms_norm(x, w)
     assert torch.equal(y[-9:], N.rms_norm(x[-9:].clone(), w)) and torch.equal(y[0], y[-1])
     assert not y[1000].any() and not y[-10].any()
+
+
+def test_forward_mode_is_refused():
+    """A tangent is never dropped: the calls say that they have no forward-mode derivative."""
+    from torch.autograd import forward_ad
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for f in (N.rms_norm, N.rms_norm_e4m3):
+            for args in ((dual(x), w), (x, dual(w)), (x, w, dual(x))):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*args)
