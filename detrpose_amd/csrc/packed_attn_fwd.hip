@@ -540,7 +540,8 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
   DP_REQUIRE(d->dim > 0 && d->dim <= 128 && d->dim % 8 == 0, "%s: head dim %d (multiples of 8 up to 128)", what, d->dim);
   DP_REQUIRE(d->scale > 0.f && d->scale < INFINITY, "%s: scale %g", what, (double)d->scale);
   DP_REQUIRE((int64_t)d->tq * d->heads < INT32_MAX - BM && (int64_t)d->tk < INT32_MAX - BM, "%s: too many rows", what);
-  DP_REQUIRE((d->cu_q && d->cu_k) || d->nseq == 0, "%s: no sequence offsets", what);
+  // without sequences too: queries are searched for behind the last offset
+  DP_REQUIRE((d->cu_q && d->cu_k) || (d->nseq == 0 && d->tq == 0), "%s: no sequence offsets", what);
   DP_REQUIRE((d->q && d->out) || d->tq == 0, "%s: no queries or output", what);
   DP_REQUIRE((d->k && d->v) || d->tk == 0, "%s: no keys or values", what);
   DP_REQUIRE(!d->out_lo || (d->dtype == DP_BF16 && d->lse && (uintptr_t)d->out_lo % 16 == 0),

@@ -691,3 +691,30 @@ def test_forward_mode_is_refused():
                 A.packed_attention(*args, cu, **kw)
         with pytest.raises(RuntimeError, match="on the GPU"):   # none of them has a tangent
             A.packed_attention(q, q, q, cu)
+
+
+def _host_desc(**kw):
+    """A descriptor of four rows at addresses that the call never gets to."""
+    from detrpose_amd import _lib
+    a = _lib.PackedAttn()
+    for n in ("q", "k", "v", "out", "cu_q", "cu_k", "dout", "dq", "dk", "dv", "lse", "ws"):
+        setattr(a, n, 4096)
+    for n in ("q", "k", "v", "o", "g"):
+        setattr(a, n + "_row", 64)
+        setattr(a, n + "_head", 32)
+    a.nseq, a.tq, a.tk, a.heads, a.kv_heads, a.dim, a.scale, a.dtype, a.ws_bytes = 1, 4, 4, 2, 2, 32, 1.0, 1, 1 << 60
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+def test_offsets_are_needed_without_sequences():
+    import ctypes as C
+    from detrpose_amd import _lib
+    lib = _lib.load()
+    for kw in (dict(cu_q=None), dict(cu_k=None), dict(cu_q=None, cu_k=None)):
+        for fill in (0, 1):
+            for fn in (lib.dp_packed_attn_fwd, lib.dp_packed_attn_bwd):
+                assert fn(C.byref(_host_desc(nseq=0, fill_tail=fill, **kw)), None) == 1000
+                assert b"no sequence offsets" in lib.dp_last_error()
+    assert lib.dp_packed_attn_fwd(C.byref(_host_desc(nseq=0, tq=0, cu_q=None, cu_k=None)), None) == 0
