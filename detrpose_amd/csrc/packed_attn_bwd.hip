@@ -753,7 +753,11 @@ extern "C" int dp_packed_attn_bwd(const dp_packed_attn* d, void* stream) {
   a.kslots = p.kslots;
   a.kshares = p.kshares;
   a.kpieces = p.kpieces;
-  DP_REQUIRE((int64_t)p.items * a.hkv + p.kshares <= UINT32_MAX / NT && (int64_t)p.kslots * a.hkv < INT32_MAX / BM, "dp_packed_attn_bwd: too many tiles");
+  // every launch's grid has less than 2^32 threads; the join of dk / dv takes dp / 4 of them a key row
+  const int64_t per = NT / ((a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128) / 4);
+  DP_REQUIRE((int64_t)p.items * a.hkv + p.kshares <= UINT32_MAX / NT && (int64_t)p.kslots * a.hkv < INT32_MAX / BM &&
+                 ((int64_t)a.tk * a.hkv + per - 1) / per <= UINT32_MAX / NT,
+             "dp_packed_attn_bwd: too many tiles");
   a.dsum = (float*)d->ws;
   a.dbias_part = a.dsum + (int64_t)d->tq * d->heads;
   a.kv_part = a.dsum + ((int64_t)d->tq * d->heads + (a.bias ? (int64_t)p.items * d->heads * d->buckets : 0) + 3) / 4 * 4;

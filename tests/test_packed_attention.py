@@ -718,3 +718,15 @@ def test_offsets_are_needed_without_sequences():
                 assert fn(C.byref(_host_desc(nseq=0, fill_tail=fill, **kw)), None) == 1000
                 assert b"no sequence offsets" in lib.dp_last_error()
     assert lib.dp_packed_attn_fwd(C.byref(_host_desc(nseq=0, tq=0, cu_q=None, cu_k=None)), None) == 0
+
+
+def test_grids_of_the_backward():
+    """A grid of 2^32 threads is refused before anything is launched, that of the keys' join too."""
+    import ctypes as C
+    from detrpose_amd import _lib
+    lib = _lib.load()
+    many = dict(nseq=1 << 20, tq=1 << 16, kv_heads=1, heads=1)
+    for kw in (dict(dim=128, tk=1 << 27), dict(dim=64, tk=1 << 28), dict(dim=8, tk=1 << 29),
+               dict(dim=8, tk=1 << 27, heads=4, kv_heads=4)):
+        assert lib.dp_packed_attn_bwd(C.byref(_host_desc(**{**many, **kw})), None) == 1000, kw
+        assert b"too many tiles" in lib.dp_last_error(), kw
