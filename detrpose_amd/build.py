@@ -124,6 +124,8 @@ def build(force: bool = False, verbose: bool = False, variant: str = "") -> str:
     stamp, flags = os.path.join(BUILD, "flags.txt"), " ".join(_flags())
     if not os.path.exists(stamp) or open(stamp).read() != flags:
         force = True
+        if os.path.exists(stamp):   # until all are compiled, the objects are of no one set of flags
+            os.remove(stamp)
     jobs = []
     objs = []
     for s in srcs:
