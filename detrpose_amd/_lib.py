@@ -91,7 +91,8 @@ class PackedAttn(C.Structure):
                 ("causal", i32), ("fill_tail", i32), ("scale", f32), ("dtype", i32),
                 ("bias", vp), ("bias_dtype", i32), ("buckets", i32), ("both", i32), ("edge", i32 * 64),
                 ("ws", vp), ("ws_bytes", i64),
-                ("dout", vp), ("g_row", i64), ("g_head", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dbias", vp)]
+                ("dout", vp), ("g_row", i64), ("g_head", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dbias", vp),
+                ("lse_lo", vp)]
 
 
 def rowmap(base=0, group=1, stride_g=0, stride_r=0) -> RowMap:

@@ -128,6 +128,8 @@ def _ptr(t):
 def _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, fill_tail):
     a = _lib.PackedAttn()
     a.q, a.k, a.v, a.out, a.lse, a.out_lo = _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(lo)
+    if lse is not None and lse.shape[0] == 2 and lse.numel():
+        a.lse_lo = lse.data_ptr() + 4 * lse.stride(0)
     (a.q_row, a.q_head), (a.k_row, a.k_head) = _strides(q), _strides(k)
     (a.v_row, a.v_head), (a.o_row, a.o_head) = _strides(v), _strides(out)
     a.cu_q, a.cu_k, a.nseq = _ptr(cu_q), _ptr(cu_k), cu_q.numel() - 1
@@ -148,7 +150,9 @@ def _forward(q, k, v, cu_q, cu_k, causal, scale, table, edges, both, out, need_l
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lib = _lib.load()
     with _lib.device_of(q):
-        lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if need_lse else None
+        lse = None   # with a bias also what its rounding left off
+        if need_lse:
+            lse = torch.empty((1 if table is None else 2, *q.shape[:2]), device=q.device, dtype=torch.float32)
         lo = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_lse and q.dtype == torch.bfloat16 else None
         a = _desc(q, k, v, out, lse, lo, cu_q, cu_k, causal, scale, table, edges, both, fill)
         nb = int(lib.dp_packed_attn_ws_bytes(C.byref(a), 0))

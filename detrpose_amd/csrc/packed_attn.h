@@ -44,7 +44,7 @@ struct alignas(16) Piece { int start, len, start2, len2, tile, w0, w1, parts, be
 struct Args {
   const void *q, *k, *v;
   void* out;
-  float* lse;
+  float *lse, *lse_lo;
   bf16_t* out_lo;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
   const int32_t *cu_q, *cu_k;
@@ -342,6 +342,22 @@ __device__ __forceinline__ void put4(T* out, bf16_t* lo, const f32x4& x) {
       for (int e = 0; e < 4; ++e) r[e] = (bf16_t)(x[e] - (float)w[e]);
       *reinterpret_cast<bf16x4*>(lo) = r;
     }
+  }
+}
+
+// The log of a row's softmax denominator, l times the exponential of m, in the backward's units: log2 without a
+// bias, natural with one. A learned bias can be far larger than the scores' differences (a mask of -1e9, the type's
+// lowest value): m + log l then rounds log l away and the backward's weights would not add up to 1, so with a bias
+// lse_lo takes what the sum's rounding left off, in log2.
+template <bool BIAS>
+__device__ __forceinline__ void put_lse(const Args& a, int64_t at, float m, float l) {
+  if (!a.lse) return;
+  if constexpr (BIAS) {
+    const float g = __logf(l), x = m + g, y = x - m;
+    a.lse[at] = l == 0.f ? INFINITY : x;
+    if (a.lse_lo) a.lse_lo[at] = l == 0.f ? 0.f : ((m - (x - y)) + (g - y)) * LOG2E;
+  } else {
+    a.lse[at] = l == 0.f ? INFINITY : m + __log2f(l);
   }
 }
 

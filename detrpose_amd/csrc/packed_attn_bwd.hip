@@ -276,7 +276,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
     D = half_sum(D);
   }
   if (ok && h == 0 && wk == 0) a.dsum[at] = D;
-  const float lse = ok ? a.lse[at] : INFINITY;
+  const float lse = ok ? a.lse[at] : INFINITY, lse_lo = BIAS && ok && a.lse_lo ? a.lse_lo[at] : 0.f;
 
   const int ks = (int)(a.k_row * sizeof(T)), vs = (int)(a.v_row * sizeof(T));
   const int koff = lane_off<T, DP>(ks, a.dim), voff = lane_off<T, DP>(vs, a.dim);
@@ -324,7 +324,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(BIAS ? (s[i] - lse) * LOG2E : fmaf(s[i], c, -lse));
+        const float p = __builtin_amdgcn_exp2f(BIAS ? fmaf(s[i] - lse, LOG2E, -lse_lo) : fmaf(s[i], c, -lse));
         s[i] = p * (dp[i] - D);
       }
       if (k32 + 32 > wmin) {
@@ -438,14 +438,15 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
   constexpr int VB = VL ? TL::bytes(BM) : 0;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* const vtile = smem + 4 * TB;
-  // lse and D of a tile's rows, two buffers
+  // lse and D of a tile's rows, and lse_lo with a bias, two buffers
+  constexpr int STATS = BIAS ? 3 : 2;
   float* lse_s = reinterpret_cast<float*>(vtile + VB);
-  float* dsum_s = lse_s + 2 * BR;
+  float *dsum_s = lse_s + 2 * BR, *lo_s = dsum_s + 2 * BR;
   const int wave = uniform(threadIdx.x >> 6);   // uniform: scalar branches below
   const int kvh = uniform(blockIdx.x % a.hkv);
   const int heads = a.hkv * a.group;
   Bias bias{};
-  if constexpr (BIAS) bias = bias_setup<T>(a, vtile + VB + 16 * BR, kvh);
+  if constexpr (BIAS) bias = bias_setup<T>(a, vtile + VB + 8 * STATS * BR, kvh);
   const int2 run = a.kv_share[blockIdx.x / a.hkv];
   const int begin = uniform(run.x), last = uniform(run.y);
   for (int piece = begin; piece <= last; ++piece) {
@@ -485,11 +486,14 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
       stage_rows<T, DP, BR>((const T*)a.q + (int64_t)(q0 + p0) * a.q_row + head * a.q_head, qs, left, at, a.dim, qoff, wave);
       stage_rows<T, DP, BR>((const T*)a.dout + (int64_t)(q0 + p0) * a.g_row + head * a.g_head, gs, left, at + TB, a.dim,
                             goff, wave);
-      // the first two waves: lse and D, one row a lane (0 past the sequence, where q, dout and p are 0 too)
-      if (wave < 2) {
-        const int64_t x = (int64_t)(q0 + p0) * heads + head;
-        const i32x4 rs = make_rsrc(wave ? a.dsum + x : a.lse + x);
-        dma4(rs, reinterpret_cast<char*>((wave ? dsum_s : lse_s) + buf * BR), lane < min(left, BR) ? lane * heads * 4 : OOB, BR);
+      // the first waves: lse, D and lse_lo, one row a lane (0 past the sequence, where q, dout and p are 0 too, and
+      // where there is no lse_lo)
+      if (wave < STATS) {
+        const bool none = wave == 2 && !a.lse_lo;
+        const float* stat = wave == 1 ? a.dsum : wave == 2 && !none ? a.lse_lo : a.lse;
+        const i32x4 rs = make_rsrc(stat + (int64_t)(q0 + p0) * heads + head);
+        dma4(rs, reinterpret_cast<char*>(lse_s + wave * 2 * BR + buf * BR),
+             lane < min(left, BR) && !none ? lane * heads * 4 : OOB, BR);
       }
     };
 
@@ -536,10 +540,12 @@ __global__ __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) void packed_bwd_kv_kern
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4 ls = *reinterpret_cast<const f32x4*>(lse_s + x0 + 8 * e);
+          f32x4 lo;
+          if constexpr (BIAS) lo = *reinterpret_cast<const f32x4*>(lo_s + x0 + 8 * e);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = s[4 * e + i];
-            s[4 * e + i] = __builtin_amdgcn_exp2f(BIAS ? (v - ls[i]) * LOG2E : fmaf(v, c, -ls[i]));
+            s[4 * e + i] = __builtin_amdgcn_exp2f(BIAS ? fmaf(v - ls[i], LOG2E, -lo[i]) : fmaf(v, c, -ls[i]));
           }
         }
         if (edge) {
@@ -694,7 +700,7 @@ int launch(const Args& a, int wk, void* dbias, int bias_f32, hipStream_t s) {
   if (a.tq > 0 || a.tk > 0)
     if (const int rc = wk > 1 ? launch_q<T, DP, W, BIAS>(a, s) : launch_q<T, DP, 1, BIAS>(a, s)) return rc;
   if (a.tk > 0) {
-    const int lds = 4 * Tile<T, DP>::bytes(BR) + (sizeof(T) == 2 && DP == 128 ? Tile<T, DP>::bytes(BM) : 0) + 16 * BR + bias_lds(a);
+    const int lds = 4 * Tile<T, DP>::bytes(BR) + (sizeof(T) == 2 && DP == 128 ? Tile<T, DP>::bytes(BM) : 0) + (BIAS ? 24 : 16) * BR + bias_lds(a);
     const auto kern = packed_bwd_kv_kernel<T, DP, BR, BIAS>;
     if (const int rc = grow_lds((const void*)kern, lds)) return rc;
     hipLaunchKernelGGL(kern, dim3(a.kshares * a.hkv), dim3(NT), lds, s, a);

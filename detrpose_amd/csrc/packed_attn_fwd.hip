@@ -223,10 +223,6 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
   }
   l = half_sum(l);
 
-  // the log of the softmax's denominator in the backward's units: log2 without, natural with a bias
-  auto lse_of = [&](float mm, float ll, float none) {
-    return ll == 0.f ? none : (BIAS ? mm + __logf(ll) : mm * c + __log2f(ll));
-  };
   auto head_row = [&](int p, int hd) { return (int64_t)(q0 + p) * heads + kvh * a.group + hd; };
   // four results of a row: the output, or this cut's part of it
   auto put = [&](int64_t at, int p, int hd, int d, f32x4 x) {
@@ -237,9 +233,10 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
               a.out_lo ? a.out_lo + at * a.dim + d : nullptr, x);
     }
   };
-  auto put_lse = [&](int64_t at, float mm, float ll) {
-    if (cuts > 1) a.part_lse[(int64_t)cut * a.tq * heads + at] = lse_of(mm, ll, -INFINITY);
-    else if (a.lse) a.lse[at] = lse_of(mm, ll, INFINITY);
+  auto put_sums = [&](int64_t at, float mm, float ll) {
+    const float mu = BIAS ? mm : mm * c;   // the maximum in lse's units
+    if (cuts > 1) a.part_lse[(int64_t)cut * a.tq * heads + at] = ll == 0.f ? -INFINITY : mu + (BIAS ? __logf(ll) : __log2f(ll));
+    else put_lse<BIAS>(a, at, mu, ll);
     if (a.splits > 1 && cut == 0) a.part_n[at] = cuts;
   };
   const bool write = it.b < a.nseq || fill_tail;
@@ -264,7 +261,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
             const int d = 32 * t + 8 * e + 4 * h;
             if (d < a.dim) put(at, pos, g, d, f32x4{o[t][4 * e], o[t][4 * e + 1], o[t][4 * e + 2], o[t][4 * e + 3]});
           }
-      if (h == 0) put_lse(at, m, l);
+      if (h == 0) put_sums(at, m, l);
     }
     if (cuts > 1) return;   // packed_join_kernel looks for NaN
     unsigned long long redo = __ballot(bad && ok);
@@ -322,7 +319,7 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
       }
       const int64_t at = head_row(rp, hd);
       if (write) put(at, rp, hd, d, sum);
-      if (d == 0) put_lse(at, top, tot);
+      if (d == 0) put_sums(at, top, tot);
       if (bad) redo[jr] = 1;
     }
     if (cuts > 1) return;
@@ -398,7 +395,7 @@ __global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
       put4<T>((T*)a.out + row * a.o_row + (at - row * heads) * a.o_head + d,
               a.out_lo ? a.out_lo + at * a.dim + d : nullptr, sum);
     }
-    if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : (BIAS ? ref + __logf(tot) : ref + __log2f(tot));
+    if (d == 0) put_lse<BIAS>(a, at, ref, tot);
   }
   if (!__ballot(bad)) return;
   // NaN: the wave's rows one by one (each wave for itself: no barrier past this point but its own)
@@ -452,7 +449,7 @@ __global__ __launch_bounds__(NT) void packed_join_row_kernel(const Args a) {
       bad |= sum[e] != sum[e];
     }
     put4<T>((T*)a.out + (int64_t)row * a.o_row + head * a.o_head + d, a.out_lo ? a.out_lo + at * a.dim + d : nullptr, sum);
-    if (a.lse && d == 0) a.lse[at] = tot == 0.f ? INFINITY : ref + (BIAS ? __logf(tot) : __log2f(tot));
+    if (d == 0) put_lse<BIAS>(a, at, ref, tot);
   }
   if (threadIdx.x < 64 && __ballot(bad)) redo_row<T>(a, row, head);
 }
@@ -546,6 +543,7 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
   DP_REQUIRE((d->k && d->v) || d->tk == 0, "%s: no keys or values", what);
   DP_REQUIRE(!d->out_lo || (d->dtype == DP_BF16 && d->lse && (uintptr_t)d->out_lo % 16 == 0),
              "%s: out_lo goes with bf16 and lse, 16-byte aligned", what);
+  DP_REQUIRE(!d->lse_lo || d->lse, "%s: lse_lo goes with lse", what);
   const int e = d->dtype == DP_BF16 ? 2 : 4;
   struct { const char* name; const void* p; int64_t row, head; } t[] = {
       {"q", d->q, d->q_row, d->q_head}, {"k", d->k, d->k_row, d->k_head}, {"v", d->v, d->v_row, d->v_head},
@@ -570,6 +568,7 @@ int dp_packed_attn_args(const dp_packed_attn* d, dppa::Args* a, const char* what
     DP_REQUIRE(d->buckets >= 2 && d->buckets <= 64 && (!d->both || d->buckets % 2 == 0) && nb >= 2, "%s: %d buckets",
                what, d->buckets);
     DP_REQUIRE(a->group * d->buckets <= 4096, "%s: %d heads a group x %d buckets", what, a->group, d->buckets);
+    a->lse_lo = d->lse_lo;
     a->bias = d->bias; a->bias_f32 = d->bias_dtype == DP_F32; a->buckets = d->buckets; a->both = d->both != 0;
     a->nedge = nb - 1;
     for (int i = 0; i < a->nedge; ++i) {

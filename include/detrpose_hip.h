@@ -775,6 +775,9 @@ typedef struct dp_packed_attn {
   const void* dout;
   int64_t g_row, g_head;
   void *dq, *dk, *dv, *dbias;
+  /* with a bias: NULL, or f32 [tq][heads] beside lse, which both directions take: what lse's rounding left off. Without
+   * it the backward's weights are off by lse's rounding, 2^-24 of the bias where that is far above the scores. */
+  float* lse_lo;
 } dp_packed_attn;
 int64_t dp_packed_attn_ws_bytes(const dp_packed_attn* d, int32_t backward);
 int dp_packed_attn_fwd(const dp_packed_attn* d, void* stream);

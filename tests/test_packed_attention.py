@@ -730,3 +730,42 @@ def test_grids_of_the_backward():
                dict(dim=8, tk=1 << 27, heads=4, kv_heads=4)):
         assert lib.dp_packed_attn_bwd(C.byref(_host_desc(**{**many, **kw})), None) == 1000, kw
         assert b"too many tiles" in lib.dp_last_error(), kw
+
+
+# A bias that is the same everywhere changes no weight. With q or k of zeros every score is exactly the bias, so the
+# reference with a table of zeros is the answer, to the same bounds, however large the bias is: the scores'
+# differences and the exponentials carry no error of its size.
+ALIKE = [(2, 2, 32, [70], [70], True), (4, 2, 64, [33, 5], [200, 1], False), (4, 1, 128, [300, 1], [300, 40], True)]
+
+
+def _alike(dtype, heads, hk, d, ql, kl, causal, bias):
+    q, k, v, dout, t = _inputs(21, dtype, heads, hk, d, ql, kl, 8)
+    for zero in ("q", "k"):
+        x = {"q": q, "k": k, zero: torch.zeros_like(q if zero == "q" else k)}
+        want = _reference(x["q"], x["k"], v, ql, kl, causal, d ** -0.5, torch.zeros_like(t), 128, not causal, dout)
+        got = _run(x["q"], x["k"], v, dout, ql, kl, torch.full_like(t, bias), causal=causal)
+        for n in want:
+            _check(got[n], want[n], (zero, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", ALIKE, ids=lambda s: f"h{s[0]}k{s[1]}d{s[2]}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bias", [-1e4, -1e9, "lowest", 1e6])
+def test_gradients_under_a_large_bias(shape, dtype, bias):
+    """Weights and their gradients where all that a query sees has one bias, small or as low as the type goes."""
+    _alike(dtype, *shape, torch.finfo(dtype).min if bias == "lowest" else bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_gradients_beside_the_lowest_bias(dtype):
+    """The lowest value hides as -inf does what stands beside other keys."""
+    ql = [150, 3]
+    q, k, v, dout, t = _inputs(22, dtype, 4, 2, 64, ql, ql, 8)
+    t[2:] = -math.inf
+    want = _reference(q, k, v, ql, ql, True, 0.125, t, 20, False, dout)
+    t[2:] = torch.finfo(dtype).min
+    got = _run(q, k, v, dout, ql, ql, t, causal=True, max_distance=20)
+    for n in want:
+        _check(got[n], want[n], n)
