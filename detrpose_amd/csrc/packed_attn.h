@@ -52,7 +52,7 @@ struct Args {
   float scale;
   // split keys (forward): key chunk at least, most chunks of one sequence, and where the parts go
   int chunk, splits;
-  float *part, *part_lse;
+  float *part, *part_m, *part_l;
   int* part_n;
   // bias
   const void* bias;

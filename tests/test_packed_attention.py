@@ -769,3 +769,20 @@ def test_gradients_beside_the_lowest_bias(dtype):
     got = _run(q, k, v, dout, ql, ql, t, causal=True, max_distance=20)
     for n in want:
         _check(got[n], want[n], n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 2, 64, [1, 2], [5000, 1300], True), (2, 1, 128, [3], [9001], True),
+                                   (4, 4, 32, [200, 3], [4100, 1700], False)], ids=lambda s: f"h{s[0]}k{s[1]}d{s[2]}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bias", [-1e4, "lowest", 1e6])
+def test_cut_keys_under_a_large_bias(shape, dtype, bias):
+    """Few queries over many keys, which are cut into parts of unequal length: each part weighs as its keys do."""
+    _alike(dtype, *shape, torch.finfo(dtype).min if bias == "lowest" else bias)
+    heads, hk, d, ql, kl, causal = shape
+    q, k, v, _, t = _inputs(23, dtype, heads, hk, d, ql, kl, 8)
+    v[kl[0] - 60:kl[0]] += 30                                # in the last part of the first sequence
+    q.zero_()
+    want = _reference(q, k, v, ql, kl, causal, d ** -0.5, torch.zeros_like(t), 128, not causal)
+    t.fill_(torch.finfo(dtype).min if bias == "lowest" else bias)
+    _check(A.packed_attention(q, k, v, _cu(ql), _cu(kl), causal=causal, bias_table=t), want["out"], "out")
