@@ -29,9 +29,18 @@ def _dense(t):
     return True
 
 
-def _holds(t):
-    """Whether a tensor stands for its .grad: a parameter, frozen or not, and every leaf that has or asks for one."""
-    return isinstance(t, torch.nn.Parameter) or (t.is_leaf and (t.requires_grad or t.grad is not None))
+def _holds(tensors):
+    """Which tensors stand for their .grad: parameters, frozen or not, and leaves that have one or ask for one. (The
+    whole list at once: hundreds of tensors are looked at in front of a few launches.)"""
+    kinds = set(map(type, tensors))
+    if kinds == {torch.nn.Parameter}:
+        return [True] * len(tensors)
+    holds = [t.requires_grad or t.grad is not None for t in tensors]
+    if True in holds:   # what a graph computed is a gradient itself
+        holds = [h and t.is_leaf for h, t in zip(holds, tensors)]
+    if kinds != {torch.Tensor}:
+        holds = [h or isinstance(t, torch.nn.Parameter) for h, t in zip(holds, tensors)]
+    return holds
 
 
 def clip_grad_norm_(parameters, max_norm, out=None):
@@ -55,9 +64,9 @@ def clip_grad_norm_(parameters, max_norm, out=None):
     if not max_norm >= 0:
         raise ValueError(f"clip_grad_norm_: max_norm {max_norm}")
     tensors = list(parameters)
-    holds = list(map(_holds, tensors))
-    if any(holds):
-        if not all(holds):
+    holds = _holds(tensors)
+    if True in holds:
+        if False in holds:
             raise ValueError(f"clip_grad_norm_: parameters and, at {holds.index(False)}, a tensor that neither is one nor "
                              "requires a gradient: pass parameters or gradients")
         grads = [g for g in (p.grad for p in tensors) if g is not None]
