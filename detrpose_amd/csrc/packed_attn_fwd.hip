@@ -233,14 +233,18 @@ __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 && DP == 128 ? 1 : 2, DP == 12
               a.out_lo ? a.out_lo + at * a.dim + d : nullptr, x);
     }
   };
+  auto lse2 = [&](float mm, float ll, float none) { return ll == 0.f ? none : mm + __log2f(ll); };
   auto put_sums = [&](int64_t at, float mm, float ll) {
-    const float mu = BIAS ? mm : mm * c;   // the maximum in lse's units
-    if (cuts > 1) {
-      // apart: under a large bias their sum as an lse would round the parts' sizes away
-      a.part_m[(int64_t)cut * a.tq * heads + at] = mu;
-      a.part_l[(int64_t)cut * a.tq * heads + at] = ll;
+    if constexpr (BIAS) {
+      if (cuts > 1) {   // apart: under a large bias one number, m + log l, would round the part's size away
+        a.part_m[(int64_t)cut * a.tq * heads + at] = mm;
+        a.part_l[(int64_t)cut * a.tq * heads + at] = ll;
+      } else {
+        put_lse<BIAS>(a, at, mm, ll);
+      }
     } else {
-      put_lse<BIAS>(a, at, mu, ll);
+      if (cuts > 1) a.part_m[(int64_t)cut * a.tq * heads + at] = lse2(mm * c, ll, -INFINITY);
+      else if (a.lse) a.lse[at] = lse2(mm * c, ll, INFINITY);
     }
     if (a.splits > 1 && cut == 0) a.part_n[at] = cuts;
   };
@@ -360,8 +364,8 @@ __device__ __forceinline__ void redo_row(const Args& a, int row, int head) {
               });
 }
 
-// rows whose keys were cut: out = sum of the parts weighted by l exp(m - the largest m), four elements
-// a thread, in the order of the cuts
+// rows whose keys were cut: out = sum of the parts weighted by l exp(m - the largest m) (without a bias m holds
+// m + log l, and l is 1), four elements a thread, in the order of the cuts
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
   constexpr int TPR = DP / 4;   // threads of a row
@@ -380,7 +384,7 @@ __global__ __launch_bounds__(NT) void packed_join_kernel(const Args a) {
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const float x = (a.part_m[i * all + at] - ref) * (BIAS ? LOG2E : 1.f);
-      const float f = __builtin_amdgcn_exp2f(x) * a.part_l[i * all + at];   // a part that saw nothing: 0
+      const float f = __builtin_amdgcn_exp2f(x) * (BIAS ? a.part_l[i * all + at] : 1.f);   // a part that saw nothing: 0
       tot += f;
       if (d < a.dim) {
         const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + (i * all + at) * a.dim + d);
@@ -424,7 +428,8 @@ __global__ __launch_bounds__(NT) void packed_join_row_kernel(const Args a) {
   const int64_t all = (int64_t)a.tq * heads, at = blockIdx.x;
   const int n = uniform(min(a.part_n[at], a.splits));
   if (n <= 1) return;
-  const float x = lane < n ? a.part_m[lane * all + at] : -INFINITY, l = lane < n ? a.part_l[lane * all + at] : 0.f;
+  const float x = lane < n ? a.part_m[lane * all + at] : -INFINITY;
+  const float l = !BIAS ? 1.f : lane < n ? a.part_l[lane * all + at] : 0.f;
   const float top = wave_max(x), ref = top == -INFINITY ? 0.f : top;
   const float f = __builtin_amdgcn_exp2f((x - ref) * (BIAS ? LOG2E : 1.f)) * l, tot = wave_sum(f);
   const int grp = threadIdx.x / TPR, d = (threadIdx.x % TPR) * 4;
@@ -479,7 +484,7 @@ static Plan plan_of(const dp_packed_attn* d) {
     chunk = (chunk + 127) / 128 * 128;
     int64_t splits = std::min<int64_t>(64, (d->tk + chunk - 1) / chunk);
     splits = std::min(splits, std::max<int64_t>(1, (few ? 64 : 4) * target / std::max<int64_t>(1, rows / per * d->kv_heads)));
-    splits = std::min(splits, std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)d->tq * d->heads * (d->dim + 2) * 4)));
+    splits = std::min(splits, std::max<int64_t>(1, ((int64_t)256 << 20) / ((int64_t)d->tq * d->heads * (d->dim + 1) * 4)));
     if (splits > 1) {
       p.chunk = (int)chunk;
       p.splits = (int)splits;
@@ -528,7 +533,7 @@ extern "C" int64_t dp_packed_attn_ws_bytes(const dp_packed_attn* d, int32_t back
   if (!d || d->heads <= 0 || d->kv_heads <= 0 || d->tq < 0 || d->tk < 0 || d->nseq < 0) return 0;
   if (!backward) {
     const Plan p = plan_of(d);
-    return p.splits > 1 ? (int64_t)d->tq * d->heads * (p.splits * ((int64_t)d->dim + 2) + 1) * 4 : 0;
+    return p.splits > 1 ? (int64_t)d->tq * d->heads * (p.splits * ((int64_t)d->dim + (d->bias ? 2 : 1)) + 1) * 4 : 0;
   }
   return dp_packed_bwd_ws_bytes(d);
 }
@@ -602,7 +607,7 @@ extern "C" int dp_packed_attn_fwd(const dp_packed_attn* d, void* stream) {
     a.part = (float*)d->ws;
     a.part_m = a.part + n * p.splits * d->dim;
     a.part_l = a.part_m + n * p.splits;
-    a.part_n = (int*)(a.part_l + n * p.splits);
+    a.part_n = (int*)(a.part_l + (d->bias ? n * p.splits : 0));
   }
   hipStream_t s = as_stream(stream);
   const int f = d->fill_tail;
