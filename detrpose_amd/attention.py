@@ -211,11 +211,13 @@ def packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     bias_table (buckets, heads), f32 or q's type: a learned bias by relative position j - position, in
     the buckets of `bucket_edges(buckets, max_distance, bidirectional)`; when bidirectional (by default:
     unless causal) keys behind the position take the upper half of the buckets, otherwise they count as
-    distance 0. It differs by head, and its gradient is summed in f32.
+    distance 0. It differs by head, and its gradient is summed in f32. Where all that a query sees has the
+    type's lowest value (or any bias that swallows the scores), its weights are equal, in the gradients too.
 
     Returns (Tq, heads, dim) of q's type; rows behind the last sequence are zeros. Differentiable (once, in
     reverse) in q, k, v and bias_table, with equal bits for equal inputs; gradients of rows behind the last sequence are
-    zeros. Scores and sums are f32; in bf16 the weights (and their gradients) are rounded to bf16 for the
+    zeros. How long walks are cut goes by the whole call's sizes, so a sequence's last bits may change with what
+    is packed beside it. Scores and sums are f32; in bf16 the weights (and their gradients) are rounded to bf16 for the
     products with v, q and k. out: the result is written here instead, rows behind the last sequence are left
     as they are; without gradients only, and in memory apart from what is read.
     Values that causal order hides from a query do not reach its output, be they inf or NaN; its gradients

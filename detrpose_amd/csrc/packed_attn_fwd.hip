@@ -8,7 +8,7 @@
 // (p stays below 256): the rescaling of O is then rare. p is rounded to bf16 for its product (by at most 2^-8
 // of itself, as the output's own rounding); the sum takes it unrounded.
 // Bound by the matrix pipe beside the exponentials: causal prompts of 8075 tokens, 32 heads x 128, 211 us, 870
-// TFLOP/s; where rows are few by HBM: 64 single tokens over 131 k keys 124 us, 4.2 TB/s.
+// TFLOP/s; where rows are few by HBM: 16 single tokens over 128 k keys 124 us, 4.2 TB/s.
 #include "packed_attn.h"
 #include <algorithm>
 
@@ -476,7 +476,7 @@ static Plan plan_of(const dp_packed_attn* d) {
   int64_t items = rows / per + d->nseq + 1;
   if (d->tk > 1024 && (few || (rows / per + 1) * d->kv_heads < 256) && d->tq > 0) {
     // about 256 blocks of few rows (a block's start costs as much as 20 tiles: 64 sequences of 2000 keys 80 us with
-    // 1024 blocks, 62 with 512, 57 with 256; 131 k ragged keys 139, 130, 133), or 512 of many; a part of the output
+    // 1024 blocks, 62 with 512, 57 with 256; 128 k ragged keys 139, 130, 133), or 512 of many; a part of the output
     // is written in f32 per cut and row, so a cut has at least 16 keys a row (splits_of)
     const int64_t target = few ? 256 : 512;
     const int64_t most_tiles = rows / per + 1;             // of one sequence

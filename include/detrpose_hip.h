@@ -739,12 +739,12 @@ int dp_maxpool2x2_pad_rb_bwd(const void* x, int64_t x_bstride, int32_t x_pstride
 
 /* Attention over packed sequences: sequence b owns query rows [cu_q[b], cu_q[b + 1]) of q / out and key
  * rows [cu_k[b], cu_k[b + 1]) of k / v (cu_*: device int32 [nseq + 1], rising, the first taken as 0;
- * values past tq / tk are cut there). Query i of lq has position i + lk - lq (the last query sits on the
- * last key); causal: it sees keys j <= position. s = scale q.k (+ bias), p = softmax over the seen
+ * values past tq / tk are cut there; both are needed where there is a query, also with nseq 0). Query i of lq has
+ * position i + lk - lq (the last query sits on the last key); causal: it sees keys j <= position. s = scale q.k (+ bias), p = softmax over the seen
  * keys (a query that sees none: zeros), out = p v. Query head h reads key head h / (heads / kv_heads).
  *  q, out [tq][heads][dim], k, v [tk][kv_heads][dim] of dtype, element strides *_row / *_head, dim
  *  contiguous, every row 16-byte aligned; dim a multiple of 8 up to 128.
- *  lse: f32 [tq][heads] (the log of the softmax's denominator, in the backward's units), or NULL.
+ *  lse: f32 [tq][heads] (the log of the softmax's denominator, in the backward's units), or NULL; lse_lo below.
  *  out_lo: NULL, or bf16 [tq][heads][dim] contiguous (dtype bf16 with lse): what out's rounding left off,
  *  out + out_lo being out to 16 bits. The backward's D = sum dout out takes it in when it is given.
  *  bias: NULL or a learned table [buckets][heads] (f32, or dtype): the bias of pair (i, j) is
