@@ -12,7 +12,7 @@
 // slot a block, and every block of the clipping launches adds all of them in the same order: no
 // atomics, so equal gradients give equal bits, and no third launch between the two.
 // Measured: 2.24 GB of reads and writes and the second read, 742 us; 368 tensors of 32.8 MB together 44 us in
-// six launches, where the host's table takes 140.
+// six launches, where the host's passes over them take 157.
 #include "common.h"
 #include <algorithm>
 #include <new>

@@ -13,8 +13,8 @@
 // ds into its own LDS bins [bucket][thread] (a 4-byte add with no other lane at that address; one add
 // per tile where the whole tile lies in one bucket); the block then adds the bins of a head's rows and
 // writes one part per block, and packed_dbias_kernel adds the parts, all in fixed orders.
-// Measured, 7055 tokens, 16 heads over 4 x 128: dq 147 us (850 TFLOP/s), dk / dv 240 (690) and 17 for their join;
-// 4031 tokens, 16 over 8 x 64 with 32 buckets: 116, 64 and 10.
+// Measured (the least of 25 launches; medians are up to 5 % above), 7055 tokens, 16 heads over 4 x 128: dq 145 us
+// (850 TFLOP/s), dk / dv 240 (690) and 17 for their join; 4031 tokens, 16 over 8 x 64 with 32 buckets: 116, 64 and 10.
 #include "packed_attn.h"
 #include <algorithm>
 

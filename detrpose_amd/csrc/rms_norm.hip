@@ -10,7 +10,7 @@
 // vector index t + TPR i, so every access of a wave is 1 KB contiguous. Rows need only their
 // element's alignment (the loads are declared so and stay 16 bytes wide); the last, partial vector
 // of a row whose length is no multiple of the vector is read and written element by element.
-// Measured, 8192 x 4096 bf16 with residual: forward 47 us and backward 47 + 6 (the sum over dw's parts) of 268 MB
+// Measured (the least of 25 launches), 8192 x 4096 bf16 with residual: forward 47 us and backward 47 + 6 (the sum over dw's parts) of 268 MB
 // each, 5.7 and 5.0 TB/s (what lies in the 256 MB behind the L2 is read faster than HBM); the e4m3 form 8.5 us
 // of 18.5 MB.
 #include "common.h"
