@@ -786,3 +786,31 @@ def test_cut_keys_under_a_large_bias(shape, dtype, bias):
     want = _reference(q, k, v, ql, kl, causal, d ** -0.5, torch.zeros_like(t), 128, not causal)
     t.fill_(torch.finfo(dtype).min if bias == "lowest" else bias)
     _check(A.packed_attention(q, k, v, _cu(ql), _cu(kl), causal=causal, bias_table=t), want["out"], "out")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_bias_without_lse_lo(dtype, monkeypatch):
+    """A caller of the C entries may leave lse_lo out: ordinary biases keep their bounds."""
+    desc = A._desc
+
+    def without(*args):
+        a = desc(*args)
+        a.lse_lo = None
+        return a
+    monkeypatch.setattr(A, "_desc", without)
+    ql, kl = [130, 1, 20], [200, 300, 20]
+    q, k, v, dout, t = _inputs(24, dtype, 4, 2, 64, ql, kl, 8)
+    got = _run(q, k, v, dout, ql, kl, t, causal=True)
+    want = _reference(q, k, v, ql, kl, True, 0.125, t, 128, False, dout)
+    for n in want:
+        _check(got[n], want[n], n)
+
+
+def test_lse_lo_needs_lse():
+    import ctypes as C
+    from detrpose_amd import _lib
+    lib = _lib.load()
+    for fn in (lib.dp_packed_attn_fwd, lib.dp_packed_attn_bwd):
+        assert fn(C.byref(_host_desc(lse=None, lse_lo=4096)), None) == 1000
+        assert b"lse_lo" in lib.dp_last_error()
